@@ -45,7 +45,15 @@ typedef enum spmvb_status {
   SPMVB_ERR_IO = 9                /* a file cannot be opened, read, written */
 } spmvb_status;
 
-typedef enum spmvb_dtype { SPMVB_F32 = 0, SPMVB_F64 = 1 } spmvb_dtype;
+/* F16 and BF16 are taken by the row-selection operators and gradient
+ * clipping (at the end of this file); the sparse matrix entry points refuse
+ * them. */
+typedef enum spmvb_dtype {
+  SPMVB_F32 = 0,
+  SPMVB_F64 = 1,
+  SPMVB_F16 = 2,
+  SPMVB_BF16 = 3
+} spmvb_dtype;
 
 /* SpMV kernels. 0..5 keep the numeric values of the reference's KernelId
  * (include/spmvbench/select.hpp:11-19); SPMVB_HYB is new (hybrid ELL+CSR). */
@@ -152,8 +160,10 @@ spmvb_status spmvb_context_create(int device, spmvb_context* out);
 spmvb_status spmvb_context_destroy(spmvb_context ctx);
 /* Synchronizes the device and reports whether any kernel launched through
  * this context gave up a bounded wait since the last check
- * (SPMVB_ERR_TIMEOUT; the word is then cleared). The host-buffer entry
- * points perform this check on their own stream before returning. */
+ * (SPMVB_ERR_TIMEOUT; the word is then cleared), or whether a row-selection
+ * operator met an index outside its range and left it out
+ * (SPMVB_ERR_INVALID_ARGUMENT; likewise). The host-buffer entry
+ * points perform the first check on their own stream before returning. */
 spmvb_status spmvb_context_check(spmvb_context ctx);
 /* Launches a kernel whose bounded wait can never be satisfied (an mbarrier
  * expecting bytes no copy delivers), with a short limit, to exercise the
@@ -491,6 +501,159 @@ spmvb_status spmvb_dist_pipeline_submit(spmvb_dist_pipeline P,
 spmvb_status spmvb_dist_pipeline_join(spmvb_dist_pipeline P, void* stream);
 spmvb_status spmvb_dist_pipeline_wait(spmvb_dist_pipeline P);
 spmvb_status spmvb_dist_pipeline_destroy(spmvb_dist_pipeline P);
+
+/* ---- row selection: embeddings and experts -------------------------------------- */
+/* Sparse products of a language model's step, whose matrix has one entry per
+ * row (tokens selecting rows of an embedding table) or k per row (tokens
+ * selecting experts) and is made on the device, anew in every step. No
+ * reference counterpart (its matrices are read from files).
+ *
+ * Conventions of this section
+ *  - dtype is SPMVB_F32, F16 or BF16; the embedding and gradient clipping
+ *    take SPMVB_F64 too. Sums are held in fp32 (fp64 for F64) and rounded
+ *    once.
+ *  - ld_* are row strides in elements, at least the row's length. Rows whose
+ *    addresses and length are multiples of 16 bytes are moved 16 bytes at a
+ *    time, others in smaller pieces.
+ *  - A negative index selects nothing: a zero row, or no contribution. An
+ *    index past the end is left out in the same way and reported by
+ *    spmvb_context_check.
+ *  - Outputs may not overlap inputs.
+ *  - Handles hold scratch memory: a handle is used by one stream at a time
+ *    (a captured graph's replays count as uses). Nothing allocates after
+ *    create and nothing synchronizes, so every call can be captured.
+ *  - Results do not depend on timing: sums have a fixed order. */
+typedef struct spmvb_embedding_st* spmvb_embedding;
+/* Scratch for the gradient of up to max_tokens rows of a rows x width table. */
+spmvb_status spmvb_embedding_create(spmvb_context ctx, int32_t rows,
+                                    int32_t width, int32_t max_tokens,
+                                    spmvb_embedding* out);
+spmvb_status spmvb_embedding_destroy(spmvb_embedding E);
+/* out[t] = scale * table[tokens[t]], t < count (any count). */
+spmvb_status spmvb_embedding_lookup(spmvb_embedding E, spmvb_dtype dtype,
+                                    int32_t count, const int32_t* d_tokens,
+                                    double scale, const void* d_table,
+                                    int64_t ld_table, void* d_out,
+                                    int64_t ld_out, void* stream);
+/* dtable[r] = scale * sum of dout[t] over the tokens t that name r (0 for
+ * rows that none names); accumulate != 0 adds to dtable instead and leaves
+ * the other rows alone. grad_dtype is dtype or SPMVB_F32. */
+spmvb_status spmvb_embedding_lookup_grad(spmvb_embedding E, spmvb_dtype dtype,
+                                         int32_t count,
+                                         const int32_t* d_tokens, double scale,
+                                         const void* d_dout, int64_t ld_dout,
+                                         spmvb_dtype grad_dtype, void* d_dtable,
+                                         int64_t ld_dtable, int accumulate,
+                                         void* stream);
+
+typedef enum spmvb_score {
+  SPMVB_SOFTMAX = 0, /* exp(l_e) / sum of exp(l) over the row's experts */
+  SPMVB_SIGMOID = 1  /* 1 / (1 + exp(-l_e))                             */
+} spmvb_score;
+/* How tokens choose experts. An expert with logit -inf or NaN is not
+ * available. With a bias the experts are ranked by score + bias, without one
+ * by their logits (the order of the scores, which saturate); equal ones go
+ * to the lowest index. With groups > 1 (a divisor of experts, neighbours
+ * together), only the groups_kept groups of the largest value can be chosen
+ * from: the sum of the group_top (1 or 2) best of score + bias in it. The
+ * weights are the chosen scores, divided by their sum if `renormalise`, times
+ * scale; the bias does not enter them. Under the softmax, a row with a NaN
+ * or +inf logit has no scores: nothing is chosen and its weights are NaN. */
+typedef struct spmvb_router_spec {
+  int32_t experts; /* 1..1024                          */
+  int32_t k;       /* 1..32, at most experts / groups * groups_kept */
+  int32_t score;   /* spmvb_score                      */
+  int32_t renormalise;
+  int32_t groups;  /* 1..32                            */
+  int32_t groups_kept;
+  int32_t group_top;
+  float scale;
+} spmvb_router_spec;
+/* The checks spmvb_router_create applies to a spec, on their own (no device
+ * needed). */
+spmvb_status spmvb_router_check(const spmvb_router_spec* spec);
+typedef struct spmvb_router_st* spmvb_router;
+spmvb_status spmvb_router_create(spmvb_context ctx,
+                                 const spmvb_router_spec* spec,
+                                 int32_t max_tokens, spmvb_router* out);
+spmvb_status spmvb_router_destroy(spmvb_router R);
+/* Chosen experts (tokens x k, best first, -1 where fewer are available) and
+ * their weights (tokens x k, fp32; 0 there). bias: experts fp32 values or
+ * NULL. d_offsets, d_order and d_position (all or none) also receive the
+ * plan of spmvb_router_plan. */
+spmvb_status spmvb_router_route(spmvb_router R, spmvb_dtype dtype,
+                                int32_t tokens, const void* d_logits,
+                                int64_t ld_logits, const float* d_bias,
+                                int32_t* d_indices, float* d_weights,
+                                int32_t* d_offsets, int32_t* d_order,
+                                int32_t* d_position, void* stream);
+/* Gradient of the weights in the logits, the choice held fixed: every entry
+ * of dlogits (tokens x experts) is written. */
+spmvb_status spmvb_router_route_grad(spmvb_router R, spmvb_dtype dtype,
+                                     int32_t tokens, const void* d_logits,
+                                     int64_t ld_logits,
+                                     const int32_t* d_indices,
+                                     const float* d_dweights, void* d_dlogits,
+                                     int64_t ld_dlogits, void* stream);
+/* The choice by expert (the routing matrix transposed): entry t * k + j goes
+ * to row position[t * k + j] of the experts' rows (-1 for no expert), expert
+ * e has rows offsets[e]..offsets[e + 1] - 1 in the order of the entries, and
+ * order[row] is the entry. offsets: experts + 1 values; order: the first
+ * offsets[experts] of tokens * k values are written, the others left. */
+spmvb_status spmvb_router_plan(spmvb_router R, int32_t tokens,
+                               const int32_t* d_indices, int32_t* d_offsets,
+                               int32_t* d_order, int32_t* d_position,
+                               void* stream);
+/* out[position[t * k + j]] = X[t]. X: tokens x width; out: out_rows x width,
+ * rows that no position names are left. */
+spmvb_status spmvb_router_dispatch(spmvb_router R, spmvb_dtype dtype,
+                                   int32_t tokens, int32_t width,
+                                   const int32_t* d_position, const void* d_X,
+                                   int64_t ld_X, int32_t out_rows, void* d_out,
+                                   int64_t ld_out, void* stream);
+/* dX[t] = sum over j of dout[position[t * k + j]]. */
+spmvb_status spmvb_router_dispatch_grad(spmvb_router R, spmvb_dtype dtype,
+                                        int32_t tokens, int32_t width,
+                                        const int32_t* d_position,
+                                        int32_t out_rows, const void* d_dout,
+                                        int64_t ld_dout, void* d_dX,
+                                        int64_t ld_dX, void* stream);
+/* out[t] = sum over j of weights[t * k + j] * Y[position[t * k + j]]. */
+spmvb_status spmvb_router_combine(spmvb_router R, spmvb_dtype dtype,
+                                  int32_t tokens, int32_t width,
+                                  const int32_t* d_position,
+                                  const float* d_weights, int32_t y_rows,
+                                  const void* d_Y, int64_t ld_Y, void* d_out,
+                                  int64_t ld_out, void* stream);
+/* dY[position[t * k + j]] = weights[t * k + j] * dout[t] (rows that no
+ * position names are left) and dweights[t * k + j] = the inner product of
+ * dout[t] and Y[position[t * k + j]] (0 for no expert). */
+spmvb_status spmvb_router_combine_grad(spmvb_router R, spmvb_dtype dtype,
+                                       int32_t tokens, int32_t width,
+                                       const int32_t* d_position,
+                                       const float* d_weights, int32_t y_rows,
+                                       const void* d_Y, int64_t ld_Y,
+                                       const void* d_dout, int64_t ld_dout,
+                                       void* d_dY, int64_t ld_dY,
+                                       float* d_dweights, void* stream);
+
+/* ---- gradient clipping ----------------------------------------------------------- */
+/* The 2-norm over many tensors at once, and their scaling by
+ * min(1, max_norm / (norm + eps)) in place. The handle holds the tensors'
+ * addresses (dense, `sizes` elements of `dtypes`; no two may overlap), which
+ * must stay valid while it is used. Squares are summed in fp64. A norm that
+ * is not finite carries on as the formula has it (NaN makes every gradient
+ * NaN). No reference counterpart. */
+typedef struct spmvb_clip_st* spmvb_clip;
+spmvb_status spmvb_clip_create(spmvb_context ctx, int32_t count,
+                               void* const* h_tensors, const int64_t* h_sizes,
+                               const spmvb_dtype* h_dtypes, spmvb_clip* out);
+spmvb_status spmvb_clip_destroy(spmvb_clip C);
+/* *d_norm (fp32, device) = the norm; the tensors are not changed. */
+spmvb_status spmvb_clip_norm(spmvb_clip C, float* d_norm, void* stream);
+/* The norm before clipping into *d_norm, then the scaling. */
+spmvb_status spmvb_clip_run(spmvb_clip C, double max_norm, double eps,
+                            float* d_norm, void* stream);
 
 #ifdef __cplusplus
 }

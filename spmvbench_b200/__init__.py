@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
-from ._lib import (BCSR, CSR_MERGE, CSR_SCALAR, CSR_VECTOR, CSR_WARP, ELL, F32, F64, HYB,
+from ._lib import (BCSR, BF16, CSR_MERGE, CSR_SCALAR, CSR_VECTOR, CSR_WARP, ELL, F16, F32, F64, HYB,
                    KERNEL_NAMES, SpmvbError, call, load)
 
 __all__ = [
@@ -25,7 +25,7 @@ __all__ = [
     "generate_vector", "row_stats", "choose_spmv", "choose_spmv_reference", "partition_rows",
     "launch_count", "gpu_available", "csr_validate", "shard_csr", "query_gpu", "kernel_name", "nccl_unique_id",
     "CSR_SCALAR", "CSR_VECTOR", "CSR_WARP", "CSR_MERGE", "ELL", "BCSR", "HYB", "F32", "F64",
-    "KERNEL_NAMES", "WORKLOADS",
+    "F16", "BF16", "KERNEL_NAMES", "WORKLOADS", "Embedding", "Router", "GradClip",
 ]
 
 # Benchmark workloads produced by generate(): id -> name.
@@ -576,3 +576,6 @@ class DistPipeline:
             self.close()
         except Exception:
             pass
+
+
+from .selection import Embedding, GradClip, Router  # noqa: E402  (needs the classes above)

@@ -20,6 +20,7 @@ STATUS = {
 }
 
 F32, F64 = 0, 1
+F16, BF16 = 2, 3  # row-selection operators and gradient clipping only
 
 # Kernel ids (values 0..5 follow the reference's KernelId).
 CSR_SCALAR, CSR_VECTOR, CSR_WARP, CSR_MERGE, ELL, BCSR, HYB = range(7)
@@ -63,6 +64,11 @@ class RowStats(C.Structure):
 class Choice(C.Structure):
     _fields_ = [("kernel", C.c_int32), ("lanes", C.c_int32), ("block_r", C.c_int32),
                 ("block_c", C.c_int32), ("rule", C.c_int32), ("reason", C.c_char * 256)]
+
+
+class RouterSpec(C.Structure):
+    _fields_ = [("experts", C.c_int32), ("k", C.c_int32), ("score", C.c_int32), ("renormalise", C.c_int32),
+                ("groups", C.c_int32), ("groups_kept", C.c_int32), ("group_top", C.c_int32), ("scale", C.c_float)]
 
 
 P = C.c_void_p
@@ -138,6 +144,28 @@ SIGNATURES = {
     "spmvb_csr_cache_read": (C.c_int, [C.c_char_p, C.POINTER(P)]),
     "spmvb_host_csr_get": (C.c_int, [P, I32P, I32P, I64P, C.POINTER(P), C.POINTER(P), C.POINTER(P)]),
     "spmvb_host_csr_free": (None, [P]),
+    "spmvb_embedding_create": (C.c_int, [P, C.c_int32, C.c_int32, C.c_int32, C.POINTER(P)]),
+    "spmvb_embedding_destroy": (C.c_int, [P]),
+    "spmvb_embedding_lookup": (C.c_int, [P, C.c_int, C.c_int32, P, C.c_double, P, C.c_int64, P, C.c_int64, P]),
+    "spmvb_embedding_lookup_grad": (C.c_int, [P, C.c_int, C.c_int32, P, C.c_double, P, C.c_int64, C.c_int, P,
+                                              C.c_int64, C.c_int, P]),
+    "spmvb_router_check": (C.c_int, [C.POINTER(RouterSpec)]),
+    "spmvb_router_create": (C.c_int, [P, C.POINTER(RouterSpec), C.c_int32, C.POINTER(P)]),
+    "spmvb_router_destroy": (C.c_int, [P]),
+    "spmvb_router_route": (C.c_int, [P, C.c_int, C.c_int32, P, C.c_int64, P, P, P, P, P, P, P]),
+    "spmvb_router_route_grad": (C.c_int, [P, C.c_int, C.c_int32, P, C.c_int64, P, P, P, C.c_int64, P]),
+    "spmvb_router_plan": (C.c_int, [P, C.c_int32, P, P, P, P, P]),
+    "spmvb_router_dispatch": (C.c_int, [P, C.c_int, C.c_int32, C.c_int32, P, P, C.c_int64, C.c_int32, P, C.c_int64, P]),
+    "spmvb_router_dispatch_grad": (C.c_int, [P, C.c_int, C.c_int32, C.c_int32, P, C.c_int32, P, C.c_int64, P,
+                                             C.c_int64, P]),
+    "spmvb_router_combine": (C.c_int, [P, C.c_int, C.c_int32, C.c_int32, P, P, C.c_int32, P, C.c_int64, P, C.c_int64,
+                                       P]),
+    "spmvb_router_combine_grad": (C.c_int, [P, C.c_int, C.c_int32, C.c_int32, P, P, C.c_int32, P, C.c_int64, P,
+                                            C.c_int64, P, C.c_int64, P, P]),
+    "spmvb_clip_create": (C.c_int, [P, C.c_int32, P, P, P, C.POINTER(P)]),
+    "spmvb_clip_destroy": (C.c_int, [P]),
+    "spmvb_clip_norm": (C.c_int, [P, P, P]),
+    "spmvb_clip_run": (C.c_int, [P, C.c_double, C.c_double, P, P]),
 }
 
 _lib = None

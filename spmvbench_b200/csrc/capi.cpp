@@ -81,7 +81,7 @@ static AddrRangeFn addr_range_fn() {
   return fn;
 }
 
-static spmvb_status check_device_ptr(const void* p, size_t bytes, int device, const char* name) {
+spmvb_status check_device_ptr(const void* p, size_t bytes, int device, const char* name) {
   if (bytes == 0) return SPMVB_OK;
   if (!p) return fail(SPMVB_ERR_INVALID_ARGUMENT, std::string(name) + " is null");
   cudaPointerAttributes at{};
@@ -219,12 +219,13 @@ spmvb_status spmvb_context_check(spmvb_context ctx) {
   if (!ctx) return fail(SPMVB_ERR_INVALID_ARGUMENT, "null context");
   DeviceGuard g(ctx->device);
   SPMVB_TRY_CUDA(cudaDeviceSynchronize());
-  int code = 0;
-  SPMVB_TRY_CUDA(cudaMemcpy(&code, ctx->err.get(), sizeof(int), cudaMemcpyDeviceToHost));
-  if (code != 0) {
-    SPMVB_TRY_CUDA(cudaMemset(ctx->err.get(), 0, sizeof(int)));
-    return fail(SPMVB_ERR_TIMEOUT, "a kernel's bounded wait gave up (device error code " + std::to_string(code) + ")");
-  }
+  int code[2] = {0, 0};
+  SPMVB_TRY_CUDA(cudaMemcpy(code, ctx->err.get(), sizeof(code), cudaMemcpyDeviceToHost));
+  if (code[0] != 0 || code[1] != 0) SPMVB_TRY_CUDA(cudaMemset(ctx->err.get(), 0, sizeof(code)));
+  if (code[0] != 0)
+    return fail(SPMVB_ERR_TIMEOUT, "a kernel's bounded wait gave up (device error code " + std::to_string(code[0]) + ")");
+  if (code[1] != 0)
+    return fail(SPMVB_ERR_INVALID_ARGUMENT, "a row-selection operator met an index out of range and left it out");
   return SPMVB_OK;
 }
 

@@ -92,7 +92,13 @@ class DevBuf {
 // Upload host bytes into a fresh zero-filled buffer of at least `cap` bytes.
 spmvb_status upload(DevBuf& dst, const void* src, size_t bytes, size_t cap);
 
-inline size_t dtype_size(spmvb_dtype d) { return d == SPMVB_F64 ? 8 : 4; }
+inline size_t dtype_size(spmvb_dtype d) {
+  return d == SPMVB_F64 ? 8 : d == SPMVB_F16 || d == SPMVB_BF16 ? 2 : 4;
+}
+
+// `p` must be device-accessible from `device` with `bytes` bytes behind it
+// (capi.cpp); `name` is what the error calls it.
+spmvb_status check_device_ptr(const void* p, size_t bytes, int device, const char* name);
 
 }  // namespace spmvb
 
@@ -101,9 +107,11 @@ struct spmvb_context_st {
   int sm_count = 0;
   int l2_bytes = 0;
   int max_smem_optin = 0;
-  // Device error word: kernels whose bounded waits give up write a non-zero
-  // code here (see spmvb_context_check).
+  // Device error words: kernels whose bounded waits give up write a non-zero
+  // code to the first, kernels that met an index out of range to the second
+  // (see spmvb_context_check).
   spmvb::DevBuf err;
+  int* index_err() const { return err.as<int>() + 1; }
 };
 
 struct spmvb_matrix_st {
