@@ -1,13 +1,31 @@
-// Routing of tokens to experts: the choice, its weights and their gradient.
+// Routing of tokens to experts: the choice, its weights and their gradient,
+// and the plan that orders the choices by expert.
 //
-// One warp per token; lane i holds the experts i * EPL .. i * EPL + EPL - 1,
-// so the lowest lane with the largest value has the lowest index. The scores
-// are computed in fp64: two experts can lie closer together than fp32
-// resolves, and the choice between them must not depend on the rounding of
-// exp.
+// The choice. One warp per token. The lanes are divided among the groups
+// (`lanes` of them to a group, a power of two) and hold EPL experts each, so the
+// order of (lane, slot) is the order of the experts. Each expert gets one
+// 32-bit key: a fixed-point value q of what it is ranked by in the high bits,
+// its slot number, descending, in the low ones. A lane sorts its keys once;
+// a choice is then one warp-wide maximum, which names the expert and breaks
+// ties by itself, and the lane that held it moves its list up.
+//
+// A row of 256 fp32 logits takes 2.9 us of HBM time for 16,384 tokens; the
+// instructions for ranking them bound the kernel, which is why the keys are
+// single words. What q stands for:
+//   no bias, 16-bit logits  the logit itself, exactly
+//   no bias, fp32 logits    its place between the row's least and largest
+//                           logit: rounded, but in order, so only equal q of
+//                           unequal logits are in doubt
+//   bias                    score + bias between the least and largest that
+//                           can occur, with an error of `tol` units at most
+// Where two neighbours in the result lie so close that the error could have
+// exchanged them (or two groups' values at the border of the kept ones), the
+// row is done again in fp64 (choose_exact): about 0.5% of the rows of 256
+// sigmoid scores. Two experts can lie closer together than fp32 resolves, and
+// the choice between them must not depend on the rounding of exp.
 #include <cmath>
 
-#include "select.cuh"
+#include "plan.cuh"
 
 namespace spmvb {
 namespace {
@@ -28,87 +46,112 @@ __device__ __forceinline__ A warp_sum(A v) {
   return v;
 }
 
-template <typename T, int EPL>
-__global__ void __launch_bounds__(kRouteThreads)
-    route_rows(spmvb_router_spec S, const T* __restrict__ logits, int64_t ld, const float* __restrict__ bias, int tokens,
-               int* __restrict__ indices, float* __restrict__ weights) {
-  const int t = blockIdx.x * (kRouteThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (t >= tokens) return;
-  const int E = S.experts, k = S.k;
-  double l[EPL], c[EPL], score[EPL];
-  bool poison = false;
-  double top = -INFINITY;
+// How a router's experts lie in a warp.
+struct RouteShape {
+  spmvb_router_spec s;
+  int per;    // experts of a group
+  int lanes;  // lanes of a group
+};
+
+// Bits of a slot's number (lane * EPL + slot), and those left for q, which an
+// fp32 sum with 2^23 rounds to an integer: 23 at most.
+constexpr int slot_bits(int epl) { return epl == 1 ? 5 : 1 + slot_bits(epl / 2); }
+constexpr int value_bits(int epl) { return slot_bits(epl) > 9 ? 32 - slot_bits(epl) : 23; }
+
+// fp32 as an int in the same order (-0 as 0).
+__device__ __forceinline__ int ordered(float v) {
+  const int b = __float_as_int(v + 0.f);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unordered(int b) { return __int_as_float(b ^ ((b >> 31) & 0x7fffffff)); }
+
+// A 16-bit float's bits in order, above 0 for every finite value.
+template <typename T>
+__device__ __forceinline__ unsigned ordered16(T v) {
+  const unsigned b = *reinterpret_cast<const uint16_t*>(&v);
+  return b & 0x8000u ? (b == 0x8000u ? 0x8000u : 0xffffu ^ b) : b | 0x8000u;
+}
+
+// Descending order of N keys (Batcher's odd-even merge sort).
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane * EPL + i;
-    l[i] = e < E ? static_cast<double>(widen(logits[t * ld + e])) : -INFINITY;
-    poison |= isnan(l[i]) || l[i] == INFINITY;
-    if (l[i] > top) top = l[i];
-  }
-  if (S.score == SPMVB_SOFTMAX) {
-    poison = __any_sync(kAll, poison);
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t a = k[i + j], b = k[i + j + q];
+            k[i + j] = max(a, b);
+            k[i + j + q] = min(a, b);
+          }
+}
+
+// The choice of one row in fp64, from its logits each time they are needed:
+// lane j returns the j-th expert, -1 for none.
+template <typename T>
+__device__ __noinline__ int choose_exact(const RouteShape& S, const T* __restrict__ row, const float* __restrict__ bias,
+                                         int epl) {
+  const int lane = threadIdx.x & 31, group = lane / S.lanes, first = (lane % S.lanes) * epl;
+  const int own = group < S.s.groups ? max(0, min(epl, S.per - first)) : 0;
+  const int e0 = group * S.per + first;
+  const bool softmax = S.s.score == SPMVB_SOFTMAX;
+  double top = -INFINITY, sum = 0;
+  if (softmax) {
+#pragma unroll 1
+    for (int i = 0; i < own; ++i) top = fmax(top, static_cast<double>(widen(row[e0 + i])));
     top = warp_max(top);
-    double sum = 0;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      score[i] = !poison && l[i] > -INFINITY ? exp(l[i] - top) : 0.0;
-      sum += score[i];
+#pragma unroll 1
+    for (int i = 0; i < own; ++i) {
+      const double l = widen(row[e0 + i]);
+      if (l > -INFINITY) sum += exp(l - top);
     }
     sum = warp_sum(sum);
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) score[i] = sum > 0 ? score[i] / sum : 0.0;
-  } else {
-    poison = false;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) score[i] = 1.0 / (1.0 + exp(-l[i]));
   }
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane * EPL + i;
-    c[i] = bias && e < E ? score[i] + static_cast<double>(bias[e]) : l[i];
-    if (poison || !(l[i] > -INFINITY) || !(c[i] > -INFINITY)) c[i] = -INFINITY;
-  }
-  if (S.groups > 1) {
-    const int per = E / S.groups;
-    double level = -INFINITY;  // of group `lane`
-    for (int g = 0; g < S.groups; ++g) {
-      double a = -INFINITY, b = -INFINITY;  // the two best
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        const int e = lane * EPL + i;
-        if (e >= E || e / per != g || !(c[i] > -INFINITY)) continue;
-        const double v = bias || S.group_top == 1 ? c[i] : score[i];
-        if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) {
-        const double a2 = __shfl_xor_sync(kAll, a, off), b2 = __shfl_xor_sync(kAll, b, off);
-        b = fmax(fmin(a, a2), fmax(b, b2));
-        a = fmax(a, a2);
-      }
-      if (lane == g) level = S.group_top == 2 && b > -INFINITY ? a + b : a;
+  const auto score = [&](double l) { return softmax ? exp(l - top) / sum : 1.0 / (1.0 + exp(-l)); };
+  const auto rank = [&](int i) -> double {
+    const double l = widen(row[e0 + i]);
+    if (!(l > -INFINITY)) return -INFINITY;
+    const double c = bias ? score(l) + static_cast<double>(bias[e0 + i]) : l;
+    return c > -INFINITY ? c : -INFINITY;
+  };
+  bool open = own > 0;
+  if (S.s.groups > 1) {
+    double a = -INFINITY, b = -INFINITY;
+#pragma unroll 1
+    for (int i = 0; i < own; ++i) {
+      double v = rank(i);
+      if (!bias && S.s.group_top == 2 && v > -INFINITY) v = score(v);
+      if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
     }
+    for (int off = S.lanes / 2; off > 0; off >>= 1) {
+      const double a2 = __shfl_xor_sync(kAll, a, off), b2 = __shfl_xor_sync(kAll, b, off);
+      b = fmax(fmin(a, a2), fmax(b, b2));
+      a = fmax(a, a2);
+    }
+    const double level = S.s.group_top == 2 && b > -INFINITY ? a + b : a;
     int better = 0;
-    for (int g = 0; g < S.groups; ++g) {
-      const double v = __shfl_sync(kAll, level, g);
-      better += v > level || (v == level && g < lane);
+    for (int g = 0; g < S.s.groups; ++g) {
+      const double v = __shfl_sync(kAll, level, g * S.lanes);
+      better += v > level || (v == level && g < group);
     }
-    const unsigned open = __ballot_sync(kAll, lane < S.groups && better < S.groups_kept);
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int e = lane * EPL + i;
-      if (e < E && !(open >> (e / per) & 1u)) c[i] = -INFINITY;
-    }
+    open = open && better < S.s.groups_kept;
   }
-  int mine = -1;  // lane j: the j-th choice, its logit and score
-  double ml = -INFINITY, ms = 0;
-  for (int j = 0; j < k; ++j) {
-    double v = c[0];
-    int at = 0;
-#pragma unroll
-    for (int i = 1; i < EPL; ++i)
-      if (c[i] > v) { v = c[i]; at = i; }
-    int e = lane * EPL + at;
+  uint64_t taken = 0;
+  int mine = -1;
+#pragma unroll 1
+  for (int j = 0; j < S.s.k; ++j) {
+    double v = -INFINITY;
+    int e = INT32_MAX;
+#pragma unroll 1
+    for (int i = 0; open && i < own; ++i) {
+      if (taken >> i & 1u) continue;
+      const double c = rank(i);
+      if (c > v) { v = c; e = e0 + i; }
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
       const double v2 = __shfl_xor_sync(kAll, v, off);
@@ -116,28 +159,287 @@ __global__ void __launch_bounds__(kRouteThreads)
       if (v2 > v || (v2 == v && e2 < e)) { v = v2; e = e2; }
     }
     if (!(v > -INFINITY)) break;
-    double le = 0, se = 0;
+    if (e >= e0 && e < e0 + own) taken |= uint64_t(1) << (e - e0);
+    if (lane == j) mine = e;
+  }
+  return mine;
+}
+
+__device__ __forceinline__ float exp_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+
+// What a warp keeps of the bias for all its rows: per expert its place on the
+// scale of q, and the scale.
+template <int EPL>
+struct BiasScale {
+  float at[EPL];  // 2^23 + 1 + (bias - least) * scale; NaN: not available
+  float scale;    // units per score
+  int zero;       // q of score + bias = 0
+  bool exact;     // no scale: every row goes to choose_exact
+};
+
+template <int EPL, int Q>
+__device__ __forceinline__ void load_bias(const RouteShape& S, const float* __restrict__ bias, int e0, int own,
+                                          BiasScale<EPL>& B) {
+  float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    B.at[i] = i < own ? __ldg(bias + e0 + i) : NAN;
+    if (B.at[i] > -INFINITY) {
+      lo = fminf(lo, B.at[i]);
+      hi = fmaxf(hi, B.at[i]);
+    }
+  }
+  lo = -warp_max(-lo);
+  hi = warp_max(hi);
+  // Scores are within [0, 1 + 2^-17].
+  B.scale = static_cast<float>((1 << Q) - 16) / (hi - lo + 1.0001f);
+  // No finite range, one that leaves q no resolution, or one that is far from 0.
+  B.exact = !(B.scale > 1.f) || !(fabsf(lo) * B.scale < 8e6f);
+  B.zero = B.exact ? 0 : __float2int_rn(-lo * B.scale) + 1;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i)
+    B.at[i] = B.at[i] > -INFINITY ? fmaf(B.at[i] - lo, B.scale, 8388609.f) : NAN;
+}
+
+// Routes one row; lane j returns its j-th choice (expert or -1) and weight.
+template <typename T, int EPL, bool Bias>
+__device__ __forceinline__ void route_row(const RouteShape& S, const T* __restrict__ row, bool whole,
+                                          const float* __restrict__ bias, const BiasScale<EPL>& B, int& mine,
+                                          float& weight) {
+  constexpr int Slots = slot_bits(EPL);
+  constexpr bool Exact16 = !Bias && sizeof(T) == 2;
+  constexpr int Shift = Exact16 ? 16 : Slots;  // key = q << Shift | (all ones - slot number)
+  constexpr int Q = value_bits(EPL);
+  const int lane = threadIdx.x & 31, group = lane / S.lanes, first = (lane % S.lanes) * EPL;
+  const int own = group < S.s.groups ? max(0, min(EPL, S.per - first)) : 0;
+  const int e0 = group * S.per + first;
+  const int k = S.s.k;
+  const bool softmax = S.s.score == SPMVB_SOFTMAX;
+
+  Pack<T, EPL * static_cast<int>(sizeof(T))> in;
+  if (whole) {  // every slot is an expert, the rows allow wide loads
+    constexpr int VB = EPL * sizeof(T) > 16 ? 16 : EPL * static_cast<int>(sizeof(T));
+    constexpr int N = Pack<T, VB>::N;
+#pragma unroll
+    for (int i = 0; i < EPL; i += N) {
+      const Pack<T, VB> p = ld_pack<T, VB>(row + lane * EPL + i);
+#pragma unroll
+      for (int q = 0; q < N; ++q) in.v[i + q] = p.v[q];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) in.v[i] = i < own ? row[e0 + i] : narrow<T, float>(-INFINITY);
+  }
+  float l[EPL], top = -INFINITY;
+  bool poison = false;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    l[i] = widen(in.v[i]);
+    poison |= !(l[i] < INFINITY);
+    top = fmaxf(top, l[i]);
+  }
+  float sum = 0.f;
+  poison = softmax && __any_sync(kAll, poison);
+  if (poison) {
+    mine = -1;
+    weight = NAN;
+    return;
+  }
+  // Scores, where the ranking or the weights need those of the whole row.
+  const bool level_scores = !Bias && S.s.groups > 1 && S.s.group_top == 2;
+  float score[EPL];
+  if (softmax) top = unordered(__reduce_max_sync(kAll, ordered(top)));
+  if (Bias || level_scores || (softmax && !S.s.renormalise)) {
+    if (softmax) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        score[i] = l[i] > -INFINITY ? exp_fast(l[i] - top) : 0.f;
+        sum += score[i];
+      }
+      sum = warp_sum(sum);
+      const float inv = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) score[i] *= inv;
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) score[i] = __fdividef(1.f, 1.f + exp_fast(fminf(-l[i], 80.f)));
+    }
+  }
+  // Keys. `tol`: units of q that two of them may be off against each other.
+  uint32_t key[EPL];
+  const uint32_t low0 = (1u << Slots) - 1u - static_cast<uint32_t>(lane * EPL);
+  const uint32_t base0 = low0 - (0x4b000000u << Shift);  // takes the exponent of 2^23 + q off
+  // A score's error, absolute: exp2 (2^-22) and its argument (1.5 * 2^-24 |l|),
+  // 1 +, and the quotient, weighted by s (1 - s) under the sigmoid: 2.6e-7.
+  // Under the softmax relative to the largest score 1 / sum: the same and the
+  // sum's own error, below 4e-6.
+  const float off = softmax ? 7.7e-6f * (sum > 0.f ? __fdividef(1.f, sum) : 0.f) + 1.2e-7f : 4.8e-7f;
+  int tol = -1;
+  bool exact = false;
+  if constexpr (Bias) {
+    tol = static_cast<int>(2.f * (off * B.scale + 1.5f)) + 1;
+    exact = B.exact;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const float f = fmaf(score[i], B.scale, B.at[i]);  // NaN: not available
+      key[i] = f > 0.f && l[i] > -INFINITY ? (__float_as_uint(f) << Shift) + (base0 - i) : 0u;
+    }
+  } else if constexpr (Exact16) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) key[i] = l[i] > -INFINITY ? ordered16(in.v[i]) << Shift | (low0 - i) : 0u;
+  } else {
+    tol = 0;
+    float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
-      if (lane * EPL + i == e) { le = l[i]; se = score[i]; c[i] = -INFINITY; }
-    le = __shfl_sync(kAll, le, e / EPL);
-    se = __shfl_sync(kAll, se, e / EPL);
-    if (lane == j) { mine = e; ml = le; ms = se; }
+      if (l[i] > -INFINITY) {
+        lo = fminf(lo, l[i]);
+        hi = fmaxf(hi, l[i]);
+      }
+    lo = unordered(__reduce_min_sync(kAll, ordered(lo)));
+    hi = unordered(__reduce_max_sync(kAll, ordered(hi)));
+    // +inf or a range past fp32: one q for all, and fp64 decides.
+    float scale = static_cast<float>((1 << Q) - 16) / (hi - lo);
+    if (!(scale < 1e30f)) scale = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const float f = scale > 0.f ? fmaf(l[i] - lo, scale, 8388609.f) : 8388609.f;
+      key[i] = l[i] > -INFINITY ? (__float_as_uint(f) << Shift) + (base0 - i) : 0u;
+    }
   }
-  if (S.renormalise) {
+  sort_keys<EPL>(key);
+  if (S.s.groups > 1) {
+    uint32_t a, b;
+    int level_tol = tol;
+    if (level_scores) {
+      a = b = 0u;
+      level_tol = static_cast<int>(4.f * (off * 8388592.f + 1.f)) + 1;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const uint32_t v = l[i] > -INFINITY ? __float_as_uint(fmaf(score[i], 8380000.f, 8388609.f)) & 0x7fffffu : 0u;
+        b = max(b, min(a, v));
+        a = max(a, v);
+      }
+    } else {
+      a = key[0] >> Shift;
+      b = S.s.group_top == 2 && EPL > 1 ? key[EPL > 1 ? 1 : 0] >> Shift : 0u;
+      if (tol > 0 && S.s.group_top == 2) level_tol = 2 * tol;
+    }
+    for (int o = S.lanes / 2; o > 0; o >>= 1) {
+      const uint32_t a2 = __shfl_xor_sync(kAll, a, o), b2 = __shfl_xor_sync(kAll, b, o);
+      b = max(min(a, a2), max(b, b2));
+      a = max(a, a2);
+    }
+    // A group of one available expert has no second score: 0 is added.
+    const int zero = Bias ? B.zero : 1;
+    const int level = a == 0u ? INT32_MIN : static_cast<int>(a) + (S.s.group_top == 1 ? 0 : b ? static_cast<int>(b) : zero);
+    int better = 0;
+    for (int g = 0; g < S.s.groups; ++g) {
+      const int v = __shfl_sync(kAll, level, g * S.lanes);
+      better += v > level || (v == level && g < group);
+    }
+    const bool kept = group < S.s.groups && better < S.s.groups_kept;
+    const int least = __reduce_min_sync(kAll, kept ? level : INT32_MAX);
+    const int next = __reduce_max_sync(kAll, kept || group >= S.s.groups ? INT32_MIN : level);
+    exact |= next > INT32_MIN && least - next <= level_tol;
+    if (!kept) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) key[i] = 0u;
+    }
+  }
+  uint32_t picked = 0u, after = 0u;  // lane j: the j-th key and the one after it
+  for (int j = 0; j <= k; ++j) {
+    const uint32_t m = __reduce_max_sync(kAll, key[0]);
+    if (lane == j) picked = m;
+    if (lane == j - 1) after = m;
+    if (m == 0u) break;
+    if (key[0] == m) {
+#pragma unroll
+      for (int i = 0; i + 1 < EPL; ++i) key[i] = key[i + 1];
+      key[EPL - 1] = 0u;
+    }
+  }
+  if (lane >= k) picked = 0u;
+  const auto expert = [&](uint32_t v) {
+    const int slot = static_cast<int>((1u << Slots) - 1u - (v & ((1u << Slots) - 1u)));
+    const int ln = slot / EPL;
+    return ln / S.lanes * S.per + (ln % S.lanes) * EPL + slot % EPL;
+  };
+  mine = picked ? expert(picked) : -1;
+  if (!Exact16 && picked && after && static_cast<int>((picked >> Shift) - (after >> Shift)) <= tol) {
+    const int other = expert(after);  // the same logit and bias: equal, and in order
+    const bool same = widen(row[mine]) == widen(row[other]) && (!Bias || bias[mine] == bias[other]);
+    exact |= !same;
+  }
+  if (__any_sync(kAll, exact)) mine = choose_exact<T>(S, row, Bias ? bias : nullptr, EPL);
+
+  const float ml = mine >= 0 ? static_cast<float>(widen(row[mine])) : -INFINITY;
+  float w = 0.f;
+  if (S.s.renormalise) {
     // Shares of the chosen scores, from a common factor taken out of them:
     // exp(l - m) under the softmax; under the sigmoid, where m <= 0,
     // exp(l - m) / (1 + exp(l)) = sigmoid(l) * exp(-m).
-    double m = warp_max(ml);
-    if (S.score == SPMVB_SIGMOID) m = fmin(m, 0.0);
-    double s = 0;
-    if (mine >= 0) s = S.score == SPMVB_SOFTMAX ? exp(ml - m) : ml > 0 ? 1.0 / (1.0 + exp(-ml)) : exp(ml - m) / (1.0 + exp(ml));
-    const double sum = warp_sum(s);
-    ms = sum > 0 ? s / sum : 0.0;
+    float m = warp_max(ml);
+    if (!softmax) m = fminf(m, 0.f);
+    if (mine >= 0)
+      w = softmax ? expf(ml - m) : ml > 0.f ? 1.f / (1.f + expf(-ml)) : expf(ml - m) / (1.f + expf(ml));
+    const float all = warp_sum(w);
+    w = all > 0.f ? w / all : 0.f;
+  } else if (mine >= 0) {
+    w = softmax ? expf(ml - top) / sum : 1.f / (1.f + expf(-ml));
   }
-  if (lane < k) {
-    indices[static_cast<int64_t>(t) * k + lane] = mine;
-    weights[static_cast<int64_t>(t) * k + lane] = poison ? NAN : static_cast<float>(mine >= 0 ? ms * S.scale : 0.0);
+  weight = w * S.s.scale;
+}
+
+// A block takes the tokens of a tile (all tiles in turn where no plan is made),
+// a warp one row at a time. With a plan it also leaves the tile's counts of
+// each expert, or, if the tile is all there is, the plan itself.
+enum class PlanPart { None, Counts, Whole };
+
+template <typename T, int EPL, bool Bias>
+__global__ void __launch_bounds__(kRouteThreads)
+    route_rows(RouteShape S, const T* __restrict__ logits, int64_t ld, bool whole, const float* __restrict__ bias,
+               int tokens, int tile_tokens, int* __restrict__ indices, float* __restrict__ weights, PlanPart part,
+               PlanView P) {
+  extern __shared__ int shared[];  // chosen[tile_entries], then the plan's
+  __shared__ int sh[kPlanWarps];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k = S.s.k, E = S.s.experts;
+  BiasScale<EPL> B{};
+  if constexpr (Bias) {
+    const int group = lane / S.lanes, first = (lane % S.lanes) * EPL;
+    load_bias<EPL, value_bits(EPL)>(S, bias, group * S.per + first,
+                                    group < S.s.groups ? max(0, min(EPL, S.per - first)) : 0, B);
+  }
+  int* counts = shared + tile_tokens * k;
+  if (part == PlanPart::Counts) {
+    for (int e = threadIdx.x; e < P.stride; e += kRouteThreads) counts[e] = 0;
+    __syncthreads();
+  }
+  const int t0 = blockIdx.x * tile_tokens, n = min(tile_tokens, tokens - t0);
+  for (int i = w; i < n; i += kRouteThreads / 32) {
+    const int64_t t = t0 + i;
+    int mine;
+    float weight;
+    route_row<T, EPL, Bias>(S, logits + t * ld, whole, bias, B, mine, weight);
+    if (lane < k) {
+      indices[t * k + lane] = mine;
+      weights[t * k + lane] = weight;
+      if (part == PlanPart::Counts && mine >= 0) atomicAdd(&counts[mine], 1);
+      if (part == PlanPart::Whole) shared[i * k + lane] = mine;
+    }
+  }
+  if (part == PlanPart::None) return;
+  __syncthreads();
+  if (part == PlanPart::Counts) {
+    for (int e = threadIdx.x; e < P.stride; e += kRouteThreads)
+      P.counts[static_cast<int64_t>(blockIdx.x) * P.stride + e] = static_cast<uint16_t>(counts[e]);
+  } else {
+    plan_alone<2>([&](int i) { return shared[i]; }, n * k, E, counts, counts + kPlanWarps * E, sh, P.offsets, P.order,
+                  P.position);
   }
 }
 
@@ -226,16 +528,39 @@ __global__ void __launch_bounds__(kRouteThreads)
   }
 }
 
+// Lanes of a group: the warp shared out among the groups, a power of two each.
+int lanes_per_group(const spmvb_router_spec& s) {
+  int lanes = 32;
+  while (lanes * s.groups > 32) lanes /= 2;
+  return lanes;
+}
+// Experts of a lane, rounded up to a power of two: at most 64, as of 1,020
+// experts in 17 groups.
+int slots_per_lane(const spmvb_router_spec& s) {
+  int slots = 1;
+  while (slots * lanes_per_group(s) < s.experts / s.groups) slots *= 2;
+  return slots;
+}
+
+int slots_for(int experts) {
+  int slots = 1;
+  while (slots * 32 < experts) slots *= 2;
+  return slots;
+}
+
 template <typename F>
-spmvb_status with_logits(spmvb_dtype d, int experts, F&& f) {
+spmvb_status with_logits(spmvb_dtype d, int slots, F&& f) {
   const auto by_lane = [&](auto tv) -> spmvb_status {
     using std::integral_constant;
-    if (experts <= 32) return f(tv, integral_constant<int, 1>{});
-    if (experts <= 64) return f(tv, integral_constant<int, 2>{});
-    if (experts <= 128) return f(tv, integral_constant<int, 4>{});
-    if (experts <= 256) return f(tv, integral_constant<int, 8>{});
-    if (experts <= 512) return f(tv, integral_constant<int, 16>{});
-    return f(tv, integral_constant<int, 32>{});
+    switch (slots) {
+      case 1: return f(tv, integral_constant<int, 1>{});
+      case 2: return f(tv, integral_constant<int, 2>{});
+      case 4: return f(tv, integral_constant<int, 4>{});
+      case 8: return f(tv, integral_constant<int, 8>{});
+      case 16: return f(tv, integral_constant<int, 16>{});
+      case 32: return f(tv, integral_constant<int, 32>{});
+    }
+    return f(tv, integral_constant<int, 64>{});
   };
   if (d == SPMVB_F32) return by_lane(float{});
   if (d == SPMVB_F16) return by_lane(__half{});
@@ -249,7 +574,7 @@ struct spmvb_router_st {
   spmvb_context ctx = nullptr;
   spmvb_router_spec spec{};
   int device = 0, max_tokens = 0;
-  spmvb::SortSpace sort;
+  spmvb::PlanSpace plan;
 };
 
 using namespace spmvb;
@@ -269,6 +594,28 @@ spmvb_status exchange_args(spmvb_router R, spmvb_dtype dtype, int tokens, int wi
 }
 
 RowSet entries_of(const void* p, int64_t n, const char* name) { return {p, n > 0, n, n, 4, name}; }
+
+// Checks a plan's outputs and fills in its view.
+spmvb_status plan_args(spmvb_router R, int tokens, const int* indices, int* offsets, int* order, int* position,
+                       PlanView* P) {
+  if (tokens < 0 || tokens > R->max_tokens)
+    return fail(SPMVB_ERR_INVALID_ARGUMENT, "tokens must be in [0, max_tokens = " + std::to_string(R->max_tokens) + "]");
+  const int64_t n = static_cast<int64_t>(tokens) * R->spec.k;
+  const RowSet idx = entries_of(indices, n, "indices"), off = entries_of(offsets, R->spec.experts + 1, "offsets"),
+               ord = entries_of(order, n, "order"), pos = entries_of(position, n, "position");
+  for (const RowSet* r : {&off, &ord, &pos}) {
+    SPMVB_TRY(check_rows(*r, R->device));
+    SPMVB_TRY(check_apart(*r, idx));
+  }
+  SPMVB_TRY(check_apart(off, ord));
+  SPMVB_TRY(check_apart(off, pos));
+  SPMVB_TRY(check_apart(ord, pos));
+  *P = plan_view(R->plan, indices, tokens, R->spec.k, R->spec.experts, R->ctx->index_err());
+  P->offsets = offsets;
+  P->order = order;
+  P->position = position;
+  return SPMVB_OK;
+}
 
 }  // namespace
 
@@ -304,7 +651,7 @@ spmvb_status spmvb_router_create(spmvb_context ctx, const spmvb_router_spec* spe
     R->device = ctx->device;
     R->spec = *spec;
     R->max_tokens = max_tokens;
-    SPMVB_TRY(R->sort.alloc(static_cast<int64_t>(max_tokens) * spec->k));
+    SPMVB_TRY(R->plan.alloc(max_tokens, spec->k, spec->experts));
     *out = R.release();
     return SPMVB_OK;
   });
@@ -323,19 +670,11 @@ spmvb_status spmvb_router_plan(spmvb_router R, int32_t tokens, const int32_t* d_
                                int32_t* d_order, int32_t* d_position, void* stream) {
   clear_error();
   if (!R) return fail(SPMVB_ERR_INVALID_ARGUMENT, "null router");
-  if (tokens < 0 || tokens > R->max_tokens)
-    return fail(SPMVB_ERR_INVALID_ARGUMENT, "tokens must be in [0, max_tokens = " + std::to_string(R->max_tokens) + "]");
-  const int dev = R->device;
-  const int64_t n = static_cast<int64_t>(tokens) * R->spec.k;
-  const RowSet idx = entries_of(d_indices, n, "indices"), offsets = entries_of(d_offsets, R->spec.experts + 1, "offsets"),
-               order = entries_of(d_order, n, "order"), position = entries_of(d_position, n, "position");
-  DeviceGuard g(dev);
-  for (const RowSet* r : {&idx, &offsets, &order, &position}) SPMVB_TRY(check_rows(*r, dev));
-  for (const RowSet* r : {&offsets, &order, &position}) SPMVB_TRY(check_apart(*r, idx));
-  for (const RowSet* r : {&order, &position}) SPMVB_TRY(check_apart(offsets, *r));
-  SPMVB_TRY(check_apart(order, position));
-  return launch_plan(R->sort, d_indices, n, R->spec.experts, d_offsets, d_order, d_position, R->ctx->index_err(),
-                     static_cast<cudaStream_t>(stream));
+  DeviceGuard g(R->device);
+  PlanView P{};
+  SPMVB_TRY(plan_args(R, tokens, d_indices, d_offsets, d_order, d_position, &P));
+  SPMVB_TRY(check_rows(entries_of(d_indices, P.entries, "indices"), R->device));
+  return launch_plan(P, false, static_cast<cudaStream_t>(stream));
 }
 
 spmvb_status spmvb_router_route(spmvb_router R, spmvb_dtype dtype, int32_t tokens, const void* d_logits,
@@ -347,8 +686,7 @@ spmvb_status spmvb_router_route(spmvb_router R, spmvb_dtype dtype, int32_t token
   const bool plan = d_offsets || d_order || d_position;
   if (plan && !(d_offsets && (tokens == 0 || (d_order && d_position))))
     return fail(SPMVB_ERR_INVALID_ARGUMENT, "offsets, order and position come together");
-  if (tokens < 0 || (plan && tokens > R->max_tokens))
-    return fail(SPMVB_ERR_INVALID_ARGUMENT, "tokens must be in [0, max_tokens = " + std::to_string(R->max_tokens) + "]");
+  if (tokens < 0) return fail(SPMVB_ERR_INVALID_ARGUMENT, "negative tokens");
   const auto& S = R->spec;
   const int dev = R->device;
   const int64_t n = static_cast<int64_t>(tokens) * S.k;
@@ -362,17 +700,39 @@ spmvb_status spmvb_router_route(spmvb_router R, spmvb_dtype dtype, int32_t token
   for (const RowSet* o : {&idx, &weights})
     for (const RowSet* r : {&logits, &bias}) SPMVB_TRY(check_apart(*o, *r));
   SPMVB_TRY(check_apart(idx, weights));
+  PlanView P{};
+  if (plan) {
+    SPMVB_TRY(plan_args(R, tokens, d_indices, d_offsets, d_order, d_position, &P));
+    for (const RowSet& o : {entries_of(d_offsets, S.experts + 1, "offsets"), entries_of(d_order, n, "order"),
+                            entries_of(d_position, n, "position")})
+      for (const RowSet* r : {&logits, &bias, &weights}) SPMVB_TRY(check_apart(o, *r));
+  }
+  const int tile = plan_tile_tokens(S.k);
+  const PlanPart part = !plan ? PlanPart::None
+                        : tokens <= tile ? PlanPart::Whole
+                        : plan_is_one_block(P) ? PlanPart::None : PlanPart::Counts;
   if (tokens > 0) {
-    SPMVB_TRY(with_logits(dtype, S.experts, [&](auto tv, auto epl) -> spmvb_status {
+    SPMVB_TRY(with_logits(dtype, slots_per_lane(S), [&](auto tv, auto epl) -> spmvb_status {
       using T = decltype(tv);
-      route_rows<T, decltype(epl)::value><<<static_cast<int>(ceil_div(tokens, kRouteThreads / 32)), kRouteThreads, 0, s>>>(
-          S, static_cast<const T*>(d_logits), ld_logits, d_bias, tokens, d_indices, d_weights);
+      constexpr int EPL = decltype(epl)::value;
+      const RouteShape shape{S, S.experts / S.groups, lanes_per_group(S)};
+      const int vb = std::min<int>(16, EPL * sizeof(T));
+      const bool whole = S.experts == 32 * EPL && access_bytes(sizeof(T), {{d_logits, ld_logits}}, vb / sizeof(T)) == vb;
+      // Without a plan a block takes a row a warp where that many blocks have room.
+      const int rows = part == PlanPart::None ? std::max(kRouteThreads / 32, static_cast<int>(ceil_div(tokens, int64_t(R->ctx->sm_count) * 4)))
+                                              : tile;
+      const size_t shared = part == PlanPart::None     ? 0
+                            : part == PlanPart::Counts ? (static_cast<size_t>(rows) * S.k + P.stride) * 4
+                                                       : (static_cast<size_t>(rows) * S.k + (kPlanWarps + 1) * S.experts) * 4;
+      const auto kernel = d_bias ? route_rows<T, EPL, true> : route_rows<T, EPL, false>;
+      kernel<<<static_cast<int>(ceil_div(tokens, rows)), kRouteThreads, shared, s>>>(
+          shape, static_cast<const T*>(d_logits), ld_logits, whole, d_bias, tokens, rows, d_indices, d_weights, part, P);
       count_launch();
       SPMVB_TRY_CUDA(cudaGetLastError());
       return SPMVB_OK;
     }));
   }
-  return plan ? spmvb_router_plan(R, tokens, d_indices, d_offsets, d_order, d_position, stream) : SPMVB_OK;
+  return plan && part != PlanPart::Whole ? launch_plan(P, part == PlanPart::Counts, s) : SPMVB_OK;
 }
 
 spmvb_status spmvb_router_route_grad(spmvb_router R, spmvb_dtype dtype, int32_t tokens, const void* d_logits,
@@ -395,7 +755,7 @@ spmvb_status spmvb_router_route_grad(spmvb_router R, spmvb_dtype dtype, int32_t 
   for (const RowSet* r : {&logits, &dlogits, &idx, &dw}) SPMVB_TRY(check_rows(*r, dev));
   for (const RowSet* r : {&logits, &idx, &dw}) SPMVB_TRY(check_apart(dlogits, *r));
   if (tokens == 0) return SPMVB_OK;
-  return with_logits(dtype, S.experts, [&](auto tv, auto epl) -> spmvb_status {
+  return with_logits(dtype, slots_for(S.experts), [&](auto tv, auto epl) -> spmvb_status {
     using T = decltype(tv);
     route_grad_rows<T, decltype(epl)::value><<<static_cast<int>(ceil_div(tokens, kRouteThreads / 32)), kRouteThreads, 0, s>>>(
         S, static_cast<const T*>(d_logits), ld_logits, tokens, d_indices, d_dweights, static_cast<T*>(d_dlogits),

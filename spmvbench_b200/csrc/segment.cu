@@ -1,5 +1,5 @@
-// Transposed products of a selection: the stable order of its entries by the
-// row they name, the expert plan made from it, and the embedding gradient.
+// The transposed product of a selection: the stable order of the tokens by the
+// row they name, and the embedding gradient made with it.
 //
 // Order. The entries are sorted by key (the row named, or n for none) with a
 // least-significant-digit radix sort, kDigitBits at a time. One pass: every
@@ -158,21 +158,6 @@ __global__ void __launch_bounds__(kSortThreads)
   }
 }
 
-// The plan from the sorted entries: order, its inverse, and the first row of
-// every expert (the first place whose key is at least it).
-__global__ void plan_finish(const uint32_t* __restrict__ keys, const int* __restrict__ vals, int64_t entries, int experts,
-                            int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ position) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i > entries) return;
-  const int key = i < entries ? static_cast<int>(keys[i]) : experts;
-  const int prev = i > 0 ? static_cast<int>(keys[i - 1]) : -1;
-  for (int e = prev + 1; e <= key && e <= experts; ++e) offsets[e] = static_cast<int>(i);
-  if (i == entries) return;
-  const int v = vals[i];
-  if (key < experts) order[i] = v;
-  position[v] = key < experts ? static_cast<int>(i) : -1;
-}
-
 // ---- embedding gradient ----------------------------------------------------------
 constexpr int kChunk = 16;
 constexpr int kGradThreads = 256;
@@ -286,21 +271,6 @@ spmvb_status sort_entries(SortSpace& space, const int* idx, int64_t count, int n
     out->keys = dk;
     out->entries = dv;
   }
-  SPMVB_TRY_CUDA(cudaGetLastError());
-  return SPMVB_OK;
-}
-
-spmvb_status launch_plan(SortSpace& space, const int* idx, int64_t entries, int experts, int* offsets, int* order,
-                         int* position, int* err, cudaStream_t s) {
-  if (entries == 0) {
-    SPMVB_TRY_CUDA(cudaMemsetAsync(offsets, 0, (static_cast<size_t>(experts) + 1) * 4, s));
-    return SPMVB_OK;
-  }
-  Sorted sorted{};
-  SPMVB_TRY(sort_entries(space, idx, entries, experts, err, s, &sorted));
-  plan_finish<<<static_cast<int>(ceil_div(entries + 1, 256)), 256, 0, s>>>(sorted.keys, sorted.entries, entries, experts,
-                                                                         offsets, order, position);
-  count_launch();
   SPMVB_TRY_CUDA(cudaGetLastError());
   return SPMVB_OK;
 }

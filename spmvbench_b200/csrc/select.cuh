@@ -183,8 +183,4 @@ spmvb_status launch_dispatch(spmvb_dtype dtype, const int* pos, int count, int k
 spmvb_status launch_combine_grad(spmvb_dtype dtype, const int* pos, const float* w, int count, int k, const RowSet& Y,
                                  const RowSet& dout, const RowSet& dY, float* dw, int* err, cudaStream_t s);
 
-// ---- expert plan (segment.cu) -----------------------------------------------------
-spmvb_status launch_plan(SortSpace& space, const int* idx, int64_t entries, int experts, int* offsets, int* order,
-                         int* position, int* err, cudaStream_t s);
-
 }  // namespace spmvb

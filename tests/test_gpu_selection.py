@@ -187,7 +187,8 @@ ROUTES = [
     (60, 4, "softmax", False, 1, 1, 1, False), (64, 6, "softmax", False, 8, 3, 1, False),
     (160, 6, "softmax", True, 8, 3, 2, True), (256, 8, "sigmoid", True, 8, 4, 2, True), (256, 8, "sigmoid", False, 8, 4, 2, False),
     (96, 32, "sigmoid", True, 32, 16, 2, True), (33, 10, "softmax", True, 3, 2, 2, False), (500, 5, "softmax", False, 5, 5, 1, True),
-    (1024, 32, "sigmoid", True, 2, 1, 1, True), (24, 24, "softmax", True, 1, 1, 1, True), (128, 1, "softmax", True, 1, 1, 1, False)]
+    (1024, 32, "sigmoid", True, 2, 1, 1, True), (24, 24, "softmax", True, 1, 1, 1, True), (128, 1, "softmax", True, 1, 1, 1, False),
+    (1020, 8, "sigmoid", True, 17, 5, 2, True), (330, 5, "softmax", False, 11, 4, 1, False)]
 
 
 def route_case(tokens, experts, bias, dtype, seed, masks=True, ties=True):
