@@ -6,15 +6,22 @@ namespace {
 
 // Up to this many tiles every block of plan_scatter adds up all tiles' counts
 // itself; beyond, plan_scan does it once.
-constexpr int kPlanOwnTiles = 512;
+constexpr int kPlanOwnTiles = 64;
 
 __global__ void __launch_bounds__(kPlanThreads) plan_counts(PlanView P) {
   __shared__ int c[kPlanMaxExperts];
   for (int e = threadIdx.x; e < P.stride; e += kPlanThreads) c[e] = 0;
   __syncthreads();
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * P.tile_entries;
-  for (int i = threadIdx.x; i < P.tile_entries && i0 + i < P.entries; i += kPlanThreads) {
-    const int e = plan_expert(P.indices[i0 + i], P.experts, P.err);
+  int x[2];  // a tile has at most 512 choices
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int i = q * kPlanThreads + threadIdx.x;
+    x[q] = i < P.tile_entries && i0 + i < P.entries ? __ldg(P.indices + i0 + i) : -1;
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int e = plan_expert(x[q], P.experts, P.err);
     if (e >= 0) atomicAdd(&c[e], 1);
   }
   __syncthreads();
@@ -80,9 +87,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_scatter(PlanView P, bool sc
   const int tile0 = blockIdx.x * P.block_tiles;
   const int64_t first = static_cast<int64_t>(tile0) * P.tile_entries;
   const int n = static_cast<int>(min(static_cast<int64_t>(P.tile_entries) * P.block_tiles, P.entries - first));
-  const auto load = [&](int i) { return plan_expert(P.indices[first + i], E, P.err); };
+  const auto load = [&](int i) { return __ldg(P.indices + first + i); };
   if (P.tiles <= P.block_tiles) {
-    plan_alone<kPlanRounds>(load, n, E, wc, total, sh, P.offsets, P.order, P.position);
+    plan_alone<kPlanRounds>(load, n, E, P.err, wc, total, sh, P.offsets, P.order, P.position);
     return;
   }
   if (scanned) {
@@ -94,25 +101,26 @@ __global__ void __launch_bounds__(kPlanThreads) plan_scatter(PlanView P, bool sc
     // 256 experts at a time: a warp takes every eighth tile, a lane eight experts.
     for (int c0 = 0; c0 < P.stride; c0 += 256) {
       const int e0 = c0 + lane * 8;
-      int b[8] = {}, a[8] = {};
+      // Two experts' sums to a word: a warp sees at most kPlanOwnTiles / 8 tiles
+      // of at most 512 choices, 2^15.
+      static_assert(kPlanOwnTiles / kPlanWarps * 512 < 65536);
+      uint32_t a[4] = {}, b[4] = {};
       if (e0 < P.stride) {
 #pragma unroll 8
         for (int t = w; t < P.tiles; t += kPlanWarps) {
-          int x[8];
-          unpack8(__ldg(reinterpret_cast<const uint4*>(P.counts + static_cast<int64_t>(t) * P.stride + e0)), x);
-          const int in = t < tile0 ? 1 : 0;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            a[q] += x[q];
-            b[q] += in ? x[q] : 0;
-          }
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(P.counts + static_cast<int64_t>(t) * P.stride + e0));
+          const uint32_t in = t < tile0 ? 0xffffffffu : 0u;
+          a[0] += v.x; b[0] += v.x & in;
+          a[1] += v.y; b[1] += v.y & in;
+          a[2] += v.z; b[2] += v.z & in;
+          a[3] += v.w; b[3] += v.w & in;
         }
       }
       int* ra = wc + w * 512 + lane * 8;
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        ra[q] = a[q];
-        ra[256 + q] = b[q];
+        ra[q] = a[q / 2] >> (q % 2 * 16) & 0xffffu;
+        ra[256 + q] = b[q / 2] >> (q % 2 * 16) & 0xffffu;
       }
       __syncthreads();
       const int e = c0 + threadIdx.x;
@@ -138,7 +146,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_scatter(PlanView P, bool sc
   }
   const int rounds = (n + kPlanThreads - 1) / kPlanThreads;
   int expert[kPlanRounds], rank[kPlanRounds];
-  plan_rank<kPlanRounds>(load, n, rounds, E, wc, expert, rank);
+  plan_rank<kPlanRounds>(load, n, rounds, E, P.err, wc, expert, rank);
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kPlanThreads) total[e] += before[e];
   __syncthreads();

@@ -50,8 +50,8 @@ __device__ __forceinline__ int plan_expert(int e, int experts, int* err) {
 // entry first + (warp * rounds + r) * 32 + lane, rank among the warp's equal
 // ones; wc[warp][expert] its count. wc must be zero.
 template <int Rounds, typename Load>
-__device__ __forceinline__ void plan_rank(Load&& load, int n, int rounds, int experts, int* wc, int (&expert)[Rounds],
-                                          int (&rank)[Rounds]) {
+__device__ __forceinline__ void plan_rank(Load&& load, int n, int rounds, int experts, int* err, int* wc,
+                                          int (&expert)[Rounds], int (&rank)[Rounds]) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int* mine = wc + w * experts;
 #pragma unroll
@@ -59,16 +59,31 @@ __device__ __forceinline__ void plan_rank(Load&& load, int n, int rounds, int ex
     const int i = (w * rounds + r) * 32 + lane;
     expert[r] = r < rounds && i < n ? load(i) : -1;
   }
+  // After all loads: the store of the report would hold the next one back.
+#pragma unroll
+  for (int r = 0; r < Rounds; ++r) expert[r] = plan_expert(expert[r], experts, err);
+  // The lanes with the same expert, from one vote a bit: a match instruction
+  // takes a microsecond for 32 different values.
+  unsigned same[Rounds];
+#pragma unroll
+  for (int r = 0; r < Rounds; ++r) {
+    if (r >= rounds) break;
+    same[r] = 0xffffffffu;
+    for (int bit = 1; bit <= experts; bit <<= 1) {
+      const bool on = expert[r] & bit;  // -1 is all ones, more than any expert
+      const unsigned vote = __ballot_sync(0xffffffffu, on);
+      same[r] &= on ? vote : ~vote;
+    }
+  }
 #pragma unroll
   for (int r = 0; r < Rounds; ++r) {
     if (r >= rounds) break;
     const int e = expert[r];
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const unsigned before = same & ((1u << lane) - 1u);
+    const unsigned before = same[r] & ((1u << lane) - 1u);
     const int base = e >= 0 ? mine[e] : 0;
     rank[r] = base + __popc(before);
     __syncwarp();
-    if (e >= 0 && before == 0) mine[e] = base + __popc(same);
+    if (e >= 0 && before == 0) mine[e] = base + __popc(same[r]);
     __syncwarp();
   }
 }
@@ -138,14 +153,14 @@ __device__ __forceinline__ void plan_place(const int* base, int* wc, int experts
 // The whole plan of at most kPlanThreads * Rounds entries by one block.
 // wc: kPlanWarps * experts ints, base: experts ints, sh: kPlanWarps ints.
 template <int Rounds, typename Load>
-__device__ __forceinline__ void plan_alone(Load&& load, int n, int experts, int* wc, int* base, int* sh,
+__device__ __forceinline__ void plan_alone(Load&& load, int n, int experts, int* err, int* wc, int* base, int* sh,
                                            int* __restrict__ offsets, int* __restrict__ order,
                                            int* __restrict__ position) {
   for (int i = threadIdx.x; i < kPlanWarps * experts; i += kPlanThreads) wc[i] = 0;
   __syncthreads();
   const int rounds = (n + kPlanThreads - 1) / kPlanThreads;
   int expert[Rounds], rank[Rounds];
-  plan_rank<Rounds>(load, n, rounds, experts, wc, expert, rank);
+  plan_rank<Rounds>(load, n, rounds, experts, err, wc, expert, rank);
   __syncthreads();
   for (int e = threadIdx.x; e < experts; e += kPlanThreads) {
     int c = 0;

@@ -1,17 +1,17 @@
 // Routing of tokens to experts: the choice, its weights and their gradient,
 // and the plan that orders the choices by expert.
 //
-// The choice. One warp per token. The lanes are divided among the groups
-// (`lanes` of them to a group, a power of two) and hold EPL experts each, so the
-// order of (lane, slot) is the order of the experts. Each expert gets one
-// 32-bit key: a fixed-point value q of what it is ranked by in the high bits,
-// its slot number, descending, in the low ones. A lane sorts its keys once;
-// a choice is then one warp-wide maximum, which names the expert and breaks
-// ties by itself, and the lane that held it moves its list up.
+// The choice. L lanes of a warp take a token (32, or 8 or 16 where that leaves a
+// lane eight experts: the tokens of a warp share the instructions that are not
+// per expert). The lanes are divided among the groups (2^lanes_log of
+// them to a group) and hold EPL experts each, so the order of (lane, slot) is
+// the order of the experts. Each expert gets one 32-bit key: a fixed-point
+// value q of what it is ranked by in the high bits, its slot number,
+// descending, in the low ones. A lane sorts its keys once; a choice is then
+// one maximum over the lanes, which names the expert and breaks ties by
+// itself, and the lane that held it moves its list up.
 //
-// A row of 256 fp32 logits takes 2.9 us of HBM time for 16,384 tokens; the
-// instructions for ranking them bound the kernel, which is why the keys are
-// single words. What q stands for:
+// What q stands for:
 //   no bias, 16-bit logits  the logit itself, exactly
 //   no bias, fp32 logits    its place between the row's least and largest
 //                           logit: rounded, but in order, so only equal q of
@@ -19,9 +19,9 @@
 //   bias                    score + bias between the least and largest that
 //                           can occur, with an error of `tol` units at most
 // Where two neighbours in the result lie so close that the error could have
-// exchanged them (or two groups' values at the border of the kept ones), the
-// row is done again in fp64 (choose_exact): about 0.5% of the rows of 256
-// sigmoid scores. Two experts can lie closer together than fp32 resolves, and
+// exchanged them, about 0.5% of the rows of 256 sigmoid scores, the two are
+// compared in fp64; a row where more than two experts or two groups' values
+// meet is done again in fp64 (route_exact). Two experts can lie closer together than fp32 resolves, and
 // the choice between them must not depend on the rounding of exp.
 #include <cmath>
 
@@ -31,6 +31,7 @@ namespace spmvb {
 namespace {
 
 constexpr int kRouteThreads = 256;
+constexpr int kRouteRows = 256;  // of a block, at most
 constexpr unsigned kAll = 0xffffffffu;
 
 template <typename A>
@@ -49,14 +50,14 @@ __device__ __forceinline__ A warp_sum(A v) {
 // How a router's experts lie in a warp.
 struct RouteShape {
   spmvb_router_spec s;
-  int per;    // experts of a group
-  int lanes;  // lanes of a group
+  int per;        // experts of a group
+  int lanes_log;  // 2^lanes_log lanes of a group
 };
 
 // Bits of a slot's number (lane * EPL + slot), and those left for q, which an
 // fp32 sum with 2^23 rounds to an integer: 23 at most.
-constexpr int slot_bits(int epl) { return epl == 1 ? 5 : 1 + slot_bits(epl / 2); }
-constexpr int value_bits(int epl) { return slot_bits(epl) > 9 ? 32 - slot_bits(epl) : 23; }
+constexpr int slot_bits(int slots) { return slots == 1 ? 0 : 1 + slot_bits(slots / 2); }
+constexpr int value_bits(int slots) { return slot_bits(slots) > 9 ? 32 - slot_bits(slots) : 23; }
 
 // fp32 as an int in the same order (-0 as 0).
 __device__ __forceinline__ int ordered(float v) {
@@ -65,12 +66,22 @@ __device__ __forceinline__ int ordered(float v) {
 }
 __device__ __forceinline__ float unordered(int b) { return __int_as_float(b ^ ((b >> 31) & 0x7fffffff)); }
 
-// A 16-bit float's bits in order, above 0 for every finite value.
+// Two 16-bit floats' bits in order (-0 as 0, NaN above infinity).
 template <typename T>
-__device__ __forceinline__ unsigned ordered16(T v) {
-  const unsigned b = *reinterpret_cast<const uint16_t*>(&v);
-  return b & 0x8000u ? (b == 0x8000u ? 0x8000u : 0xffffu ^ b) : b | 0x8000u;
+__device__ __forceinline__ uint32_t ordered_pair(T a, T b) {
+  uint32_t w;
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 v = __hadd2(__halves2half2(a, b), __halves2half2(__half(0.f), __half(0.f)));
+    w = *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __hadd2(__halves2bfloat162(a, b), __halves2bfloat162(__nv_bfloat16(0.f), __nv_bfloat16(0.f)));
+    w = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return w ^ ((w >> 15 & 0x00010001u) * 0xffffu | 0x80008000u);
 }
+// The infinities' places in that order: -inf is ~inf.
+template <typename T>
+constexpr uint32_t kInf16 = std::is_same_v<T, __half> ? 0xfc00u : 0xff80u;
 
 // Descending order of N keys (Batcher's odd-even merge sort).
 template <int N>
@@ -90,44 +101,62 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
           }
 }
 
-// The choice of one row in fp64, from its logits each time they are needed:
-// lane j returns the j-th expert, -1 for none.
-template <typename T>
-__device__ __noinline__ int choose_exact(const RouteShape& S, const T* __restrict__ row, const float* __restrict__ bias,
-                                         int epl) {
-  const int lane = threadIdx.x & 31, group = lane / S.lanes, first = (lane % S.lanes) * epl;
-  const int own = group < S.s.groups ? max(0, min(epl, S.per - first)) : 0;
+// Shares of the chosen scores (lane j's logit l, -inf for none) in the chosen
+// sum, from a common factor taken out of them: exp(l - m) under the softmax;
+// under the sigmoid, where m <= 0, exp(l - m) / (1 + exp(l)) = sigmoid(l) * exp(-m).
+__device__ __forceinline__ double chosen_share(double l, bool softmax) {
+  double m = warp_max(l);
+  if (!softmax) m = fmin(m, 0.0);
+  double w = 0;
+  if (l > -INFINITY) w = softmax ? exp(l - m) : l > 0 ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / (1.0 + exp(l));
+  const double all = warp_sum(w);
+  return all > 0 ? w / all : 0.0;
+}
+
+// One row in fp64, by a warp: lane j returns the j-th expert (-1 for none) and
+// its weight. Out of line, so that its registers are the kernel's only while
+// it runs.
+template <typename T, int EPL>
+__device__ __noinline__ int route_exact(const RouteShape& S, const T* __restrict__ row,
+                                        const float* __restrict__ bias, float& weight) {
+  const int lane = threadIdx.x & 31, group = lane >> S.lanes_log, first = (lane & ((1 << S.lanes_log) - 1)) * EPL;
+  const int own = group < S.s.groups ? max(0, min(EPL, S.per - first)) : 0;
   const int e0 = group * S.per + first;
   const bool softmax = S.s.score == SPMVB_SOFTMAX;
-  double top = -INFINITY, sum = 0;
-  if (softmax) {
-#pragma unroll 1
-    for (int i = 0; i < own; ++i) top = fmax(top, static_cast<double>(widen(row[e0 + i])));
-    top = warp_max(top);
-#pragma unroll 1
-    for (int i = 0; i < own; ++i) {
-      const double l = widen(row[e0 + i]);
-      if (l > -INFINITY) sum += exp(l - top);
-    }
-    sum = warp_sum(sum);
+  double l[EPL], c[EPL], top = -INFINITY, sum = 0;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    l[i] = i < own ? static_cast<double>(widen(row[e0 + i])) : -INFINITY;
+    c[i] = l[i];
+    top = fmax(top, l[i]);
   }
-  const auto score = [&](double l) { return softmax ? exp(l - top) / sum : 1.0 / (1.0 + exp(-l)); };
-  const auto rank = [&](int i) -> double {
-    const double l = widen(row[e0 + i]);
-    if (!(l > -INFINITY)) return -INFINITY;
-    const double c = bias ? score(l) + static_cast<double>(bias[e0 + i]) : l;
-    return c > -INFINITY ? c : -INFINITY;
-  };
+  if (softmax) top = warp_max(top);
+  // Rolled up: a row in doubt comes alone, and the code has to be fetched first.
+#pragma unroll 2
+  for (int i = 0; i < EPL; ++i) {
+    if (!(l[i] > -INFINITY)) continue;
+    c[i] = softmax ? exp(l[i] - top) : 1.0 / (1.0 + exp(-l[i]));
+    sum += c[i];
+  }
+  if (softmax) {
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (l[i] > -INFINITY) c[i] /= sum;
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    if (bias && i < own) c[i] += static_cast<double>(bias[e0 + i]);
+    if (!(l[i] > -INFINITY) || !(c[i] > -INFINITY)) c[i] = -INFINITY;
+  }
   bool open = own > 0;
   if (S.s.groups > 1) {
     double a = -INFINITY, b = -INFINITY;
-#pragma unroll 1
-    for (int i = 0; i < own; ++i) {
-      double v = rank(i);
-      if (!bias && S.s.group_top == 2 && v > -INFINITY) v = score(v);
-      if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      if (c[i] > a) { b = a; a = c[i]; } else if (c[i] > b) { b = c[i]; }
     }
-    for (int off = S.lanes / 2; off > 0; off >>= 1) {
+    for (int off = 1 << S.lanes_log >> 1; off > 0; off >>= 1) {
       const double a2 = __shfl_xor_sync(kAll, a, off), b2 = __shfl_xor_sync(kAll, b, off);
       b = fmax(fmin(a, a2), fmax(b, b2));
       a = fmax(a, a2);
@@ -135,33 +164,45 @@ __device__ __noinline__ int choose_exact(const RouteShape& S, const T* __restric
     const double level = S.s.group_top == 2 && b > -INFINITY ? a + b : a;
     int better = 0;
     for (int g = 0; g < S.s.groups; ++g) {
-      const double v = __shfl_sync(kAll, level, g * S.lanes);
+      const double v = __shfl_sync(kAll, level, g << S.lanes_log);
       better += v > level || (v == level && g < group);
     }
     open = open && better < S.s.groups_kept;
   }
-  uint64_t taken = 0;
+  // Ranked by the values' bits, as integers in the same order; 0: not there.
+  uint64_t key[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const double v = (bias ? c[i] : l[i]) + 0.0;  // -0 as 0
+    const int64_t bits = __double_as_longlong(v);
+    key[i] = open && v > -INFINITY ? static_cast<uint64_t>(bits) ^ (static_cast<uint64_t>(bits >> 63) | (1ull << 63)) : 0ull;
+  }
   int mine = -1;
 #pragma unroll 1
   for (int j = 0; j < S.s.k; ++j) {
-    double v = -INFINITY;
-    int e = INT32_MAX;
-#pragma unroll 1
-    for (int i = 0; open && i < own; ++i) {
-      if (taken >> i & 1u) continue;
-      const double c = rank(i);
-      if (c > v) { v = c; e = e0 + i; }
-    }
+    uint64_t v = 0;
+    int at = 0;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      const double v2 = __shfl_xor_sync(kAll, v, off);
-      const int e2 = __shfl_xor_sync(kAll, e, off);
-      if (v2 > v || (v2 == v && e2 < e)) { v = v2; e = e2; }
-    }
-    if (!(v > -INFINITY)) break;
-    if (e >= e0 && e < e0 + own) taken |= uint64_t(1) << (e - e0);
+    for (int i = 0; i < EPL; ++i)
+      if (key[i] > v) { v = key[i]; at = i; }
+    const uint32_t high = __reduce_max_sync(kAll, static_cast<uint32_t>(v >> 32));
+    if (high == 0u) break;
+    const uint32_t low = __reduce_max_sync(kAll, v >> 32 == high ? static_cast<uint32_t>(v) : 0u);
+    // The lowest lane that holds the largest value has the lowest index.
+    const int from = __ffs(__ballot_sync(kAll, v == (static_cast<uint64_t>(high) << 32 | low))) - 1;
+    const int e = __shfl_sync(kAll, e0 + at, from);
     if (lane == j) mine = e;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (lane == from && i == at) key[i] = 0ull;
   }
+  const double ml = mine >= 0 ? static_cast<double>(widen(row[mine])) : -INFINITY;
+  double w = 0;
+  if (S.s.renormalise)
+    w = chosen_share(ml, softmax);
+  else if (mine >= 0)
+    w = softmax ? exp(ml - top) / sum : 1.0 / (1.0 + exp(-ml));
+  weight = static_cast<float>(w * S.s.scale);
   return mine;
 }
 
@@ -171,52 +212,91 @@ __device__ __forceinline__ float exp_fast(float x) {
   return r;
 }
 
-// What a warp keeps of the bias for all its rows: per expert its place on the
-// scale of q, and the scale.
-template <int EPL>
-struct BiasScale {
-  float at[EPL];  // 2^23 + 1 + (bias - least) * scale; NaN: not available
-  float scale;    // units per score
-  int zero;       // q of score + bias = 0
-  bool exact;     // no scale: every row goes to choose_exact
-};
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
-template <int EPL, int Q>
-__device__ __forceinline__ void load_bias(const RouteShape& S, const float* __restrict__ bias, int e0, int own,
-                                          BiasScale<EPL>& B) {
-  float lo = INFINITY, hi = -INFINITY;
+// Maxima and sums over the L lanes of a row.
+template <int L>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  if constexpr (L == 32) return __reduce_max_sync(kAll, v);
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    B.at[i] = i < own ? __ldg(bias + e0 + i) : NAN;
-    if (B.at[i] > -INFINITY) {
-      lo = fminf(lo, B.at[i]);
-      hi = fmaxf(hi, B.at[i]);
+  for (int off = L / 2; off > 0; off >>= 1) v = max(v, __shfl_xor_sync(kAll, v, off));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ int row_max(int v) {
+  if constexpr (L == 32) return __reduce_max_sync(kAll, v);
+#pragma unroll
+  for (int off = L / 2; off > 0; off >>= 1) v = max(v, __shfl_xor_sync(kAll, v, off));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int off = L / 2; off > 0; off >>= 1) v += __shfl_xor_sync(kAll, v, off);
+  return v;
+}
+template <int L>
+__device__ __forceinline__ bool row_any(bool v) {
+  const unsigned all = __ballot_sync(kAll, v);
+  if constexpr (L == 32) return all != 0u;
+  return (all >> (threadIdx.x & 31 & ~(L - 1)) & ((1u << (L & 31)) - 1u)) != 0u;
+}
+
+// What the biases are on the scale of q, for a block's rows.
+struct BiasScale {
+  const float* at;  // per slot 2^23 + 1 + (bias - least) * scale; NaN: not available
+  float scale;      // units per score
+  int zero;         // q of score + bias = 0
+  bool exact;       // no scale: every row goes to route_exact
+};
+// Rows of the slots' table: 16-byte words that fall on different banks.
+constexpr int bias_row(int epl) { return epl >= 4 ? epl + 4 : epl; }
+
+template <int L, int EPL>
+__device__ __forceinline__ BiasScale load_bias(const RouteShape& S, const float* __restrict__ bias, float* table) {
+  const int lane = threadIdx.x & 31;
+  float lo = INFINITY, hi = -INFINITY;
+  for (int e = lane; e < S.s.experts; e += 32) {
+    const float b = __ldg(bias + e);
+    if (b > -INFINITY) {
+      lo = fminf(lo, b);
+      hi = fmaxf(hi, b);
     }
   }
   lo = -warp_max(-lo);
   hi = warp_max(hi);
+  BiasScale B;
   // Scores are within [0, 1 + 2^-17].
-  B.scale = static_cast<float>((1 << Q) - 16) / (hi - lo + 1.0001f);
+  B.scale = static_cast<float>((1 << value_bits(L * EPL)) - 16) / (hi - lo + 1.0001f);
   // No finite range, one that leaves q no resolution, or one that is far from 0.
   B.exact = !(B.scale > 1.f) || !(fabsf(lo) * B.scale < 8e6f);
   B.zero = B.exact ? 0 : __float2int_rn(-lo * B.scale) + 1;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i)
-    B.at[i] = B.at[i] > -INFINITY ? fmaf(B.at[i] - lo, B.scale, 8388609.f) : NAN;
+  for (int i = threadIdx.x; i < L * EPL; i += kRouteThreads) {
+    const int ln = i / EPL, e = (ln >> S.lanes_log) * S.per + (ln & ((1 << S.lanes_log) - 1)) * EPL + i % EPL;
+    const int last = min(((ln >> S.lanes_log) + 1) * S.per, S.s.experts);  // of the lane's group
+    const float b = e < last ? __ldg(bias + e) : NAN;
+    table[ln * bias_row(EPL) + i % EPL] = b > -INFINITY ? fmaf(b - lo, B.scale, 8388609.f) : NAN;
+  }
+  B.at = table;
+  return B;
 }
 
-// Routes one row; lane j returns its j-th choice (expert or -1) and weight.
-template <typename T, int EPL, bool Bias>
-__device__ __forceinline__ void route_row(const RouteShape& S, const T* __restrict__ row, bool whole,
-                                          const float* __restrict__ bias, const BiasScale<EPL>& B, int& mine,
-                                          float& weight) {
-  constexpr int Slots = slot_bits(EPL);
+// Routes the row of these L lanes; lane j returns its j-th choice (expert or
+// -1) and weight. `list`: this lane's column of a 32-wide array of list_depth
+// rows, the last of them 0. True: the result is in doubt.
+constexpr int list_depth(int epl) { return epl <= 8 ? epl + 1 : 0; }
+template <typename T, int L, int EPL, bool Bias>
+__device__ __forceinline__ bool route_row(const RouteShape& S, const T* __restrict__ row, bool whole, const float* __restrict__ bias, const BiasScale& B,
+                                          uint32_t* list, int& mine, float& weight) {
+  constexpr int Slots = slot_bits(L * EPL);
   constexpr bool Exact16 = !Bias && sizeof(T) == 2;
   constexpr int Shift = Exact16 ? 16 : Slots;  // key = q << Shift | (all ones - slot number)
-  constexpr int Q = value_bits(EPL);
-  const int lane = threadIdx.x & 31, group = lane / S.lanes, first = (lane % S.lanes) * EPL;
-  const int own = group < S.s.groups ? max(0, min(EPL, S.per - first)) : 0;
-  const int e0 = group * S.per + first;
+  constexpr int Q = value_bits(L * EPL);
+  const int lane = threadIdx.x & (L - 1), group = lane >> S.lanes_log, first = (lane & ((1 << S.lanes_log) - 1)) * EPL;
   const int k = S.s.k;
   const bool softmax = S.s.score == SPMVB_SOFTMAX;
 
@@ -231,105 +311,135 @@ __device__ __forceinline__ void route_row(const RouteShape& S, const T* __restri
       for (int q = 0; q < N; ++q) in.v[i + q] = p.v[q];
     }
   } else {
+    const int own = group < S.s.groups ? max(0, min(EPL, S.per - first)) : 0;
+    const T* from = row + group * S.per + first;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) in.v[i] = i < own ? row[e0 + i] : narrow<T, float>(-INFINITY);
+    for (int i = 0; i < EPL; ++i) in.v[i] = i < own ? __ldg(from + i) : narrow<T, float>(-INFINITY);
   }
-  float l[EPL], top = -INFINITY;
-  bool poison = false;
+  float l[EPL];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    l[i] = widen(in.v[i]);
-    poison |= !(l[i] < INFINITY);
-    top = fmaxf(top, l[i]);
-  }
-  float sum = 0.f;
-  poison = softmax && __any_sync(kAll, poison);
-  if (poison) {
-    mine = -1;
-    weight = NAN;
-    return;
-  }
-  // Scores, where the ranking or the weights need those of the whole row.
-  const bool level_scores = !Bias && S.s.groups > 1 && S.s.group_top == 2;
-  float score[EPL];
-  if (softmax) top = unordered(__reduce_max_sync(kAll, ordered(top)));
-  if (Bias || level_scores || (softmax && !S.s.renormalise)) {
-    if (softmax) {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        score[i] = l[i] > -INFINITY ? exp_fast(l[i] - top) : 0.f;
-        sum += score[i];
-      }
-      sum = warp_sum(sum);
-      const float inv = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) score[i] *= inv;
-    } else {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) score[i] = __fdividef(1.f, 1.f + exp_fast(fminf(-l[i], 80.f)));
-    }
-  }
-  // Keys. `tol`: units of q that two of them may be off against each other.
+  for (int i = 0; i < EPL; ++i) l[i] = widen(in.v[i]);
   uint32_t key[EPL];
   const uint32_t low0 = (1u << Slots) - 1u - static_cast<uint32_t>(lane * EPL);
-  const uint32_t base0 = low0 - (0x4b000000u << Shift);  // takes the exponent of 2^23 + q off
-  // A score's error, absolute: exp2 (2^-22) and its argument (1.5 * 2^-24 |l|),
+  constexpr uint32_t Least = Exact16 ? ((0xffffu ^ kInf16<T>) + 1u) << 16 : 1u;  // key of an available expert
+  // Under the softmax a NaN or +inf leaves the row without scores.
+  bool poison = false, exact = false;
+  if constexpr (Exact16) {
+#pragma unroll
+    for (int i = 0; i < EPL; i += 2) {
+      const uint32_t o = ordered_pair<T>(in.v[i], in.v[i + 1 < EPL ? i + 1 : i]);
+      key[i] = (o << 16) + (low0 - i);
+      if (i + 1 < EPL) key[i + 1] = (o & 0xffff0000u) + (low0 - (i + 1));
+    }
+    sort_keys<EPL>(key);
+    if (softmax)
+      poison = row_any<L>(key[0] >= kInf16<T> << 16);
+    else
+      exact = key[0] > (kInf16<T> << 16 | 0xffffu);  // NaN: not available
+  } else if (softmax) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) poison |= !(l[i] < INFINITY);
+    poison = row_any<L>(poison);
+  }
+  // The row's largest logit and sum of exponentials, where the ranking or the
+  // weights need the scores of the whole row.
+  const bool level_scores = !Bias && S.s.groups > 1 && S.s.group_top == 2;
+  float top = -INFINITY, sum = 0.f, inv = 0.f;
+  if (softmax && (Bias || level_scores || !S.s.renormalise)) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) top = fmaxf(top, l[i]);
+    top = unordered(row_max<L>(ordered(top)));
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) sum += l[i] > -INFINITY ? exp_fast(l[i] - top) : 0.f;
+    sum = row_sum<L>(sum);
+    inv = sum > 0.f ? reciprocal(sum) : 0.f;
+  }
+  // Scores, NaN where there is none.
+  const auto scores = [&](float (&v)[EPL]) {
+    if (softmax) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) v[i] = l[i] > -INFINITY ? exp_fast(l[i] - top) * inv : NAN;
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) v[i] = l[i] > -INFINITY ? reciprocal(1.f + exp_fast(-l[i])) : NAN;
+    }
+  };
+  // `tol`: units of q that two of them may be off against each other. A
+  // score's error, absolute: exp2 (2^-22) and its argument (1.5 * 2^-24 |l|),
   // 1 +, and the quotient, weighted by s (1 - s) under the sigmoid: 2.6e-7.
   // Under the softmax relative to the largest score 1 / sum: the same and the
   // sum's own error, below 4e-6.
-  const float off = softmax ? 7.7e-6f * (sum > 0.f ? __fdividef(1.f, sum) : 0.f) + 1.2e-7f : 4.8e-7f;
+  const float off = softmax ? 7.7e-6f * inv + 1.2e-7f : 2.7e-7f;
   int tol = -1;
-  bool exact = false;
+  uint32_t sa = 0u, sb = 0u;  // the two best scores on q's scale, for level_scores
   if constexpr (Bias) {
+    const uint32_t base0 = low0 - (0x4b000000u << Shift);  // takes the exponent of 2^23 + q off
     tol = static_cast<int>(2.f * (off * B.scale + 1.5f)) + 1;
     exact = B.exact;
+    float v[EPL];
+    scores(v);
+    constexpr int VB = EPL >= 4 ? 16 : EPL * 4;
+    constexpr int N = VB / 4;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const float f = fmaf(score[i], B.scale, B.at[i]);  // NaN: not available
-      key[i] = f > 0.f && l[i] > -INFINITY ? (__float_as_uint(f) << Shift) + (base0 - i) : 0u;
+    for (int i = 0; i < EPL; i += N) {
+      const Pack<float, VB> at = *reinterpret_cast<const Pack<float, VB>*>(B.at + lane * bias_row(EPL) + i);
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const float f = fmaf(v[i + q], B.scale, at.v[q]);  // NaN: not available
+        key[i + q] = f > 0.f ? (__float_as_uint(f) << Shift) + (base0 - (i + q)) : 0u;
+      }
     }
-  } else if constexpr (Exact16) {
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) key[i] = l[i] > -INFINITY ? ordered16(in.v[i]) << Shift | (low0 - i) : 0u;
+    sort_keys<EPL>(key);
   } else {
-    tol = 0;
-    float lo = INFINITY, hi = -INFINITY;
+    if (level_scores) {
+      float v[EPL];
+      scores(v);
 #pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (l[i] > -INFINITY) {
-        lo = fminf(lo, l[i]);
+      for (int i = 0; i < EPL; ++i) {
+        const float f = fmaf(v[i], 8380000.f, 8388609.f);
+        const uint32_t u = f > 0.f ? __float_as_uint(f) & 0x7fffffu : 0u;
+        sb = max(sb, min(sa, u));
+        sa = max(sa, u);
+      }
+    }
+    if constexpr (!Exact16) {
+      const uint32_t base0 = low0 - (0x4b000000u << Shift);
+      tol = 0;
+      float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        lo = fminf(lo, l[i] > -INFINITY ? l[i] : INFINITY);
         hi = fmaxf(hi, l[i]);
       }
-    lo = unordered(__reduce_min_sync(kAll, ordered(lo)));
-    hi = unordered(__reduce_max_sync(kAll, ordered(hi)));
-    // +inf or a range past fp32: one q for all, and fp64 decides.
-    float scale = static_cast<float>((1 << Q) - 16) / (hi - lo);
-    if (!(scale < 1e30f)) scale = 0.f;
+      lo = -unordered(row_max<L>(ordered(-lo)));
+      hi = unordered(row_max<L>(ordered(hi)));
+      // Equal logits, +inf or a range past fp32: one q for all, and fp64
+      // decides where they differ.
+      float scale = __fdividef(static_cast<float>((1 << Q) - 16), hi - lo);
+      if (!(scale > 0.f) || !(scale < 1e30f)) scale = 0.f;
+      if (scale == 0.f) lo = 0.f;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const float f = scale > 0.f ? fmaf(l[i] - lo, scale, 8388609.f) : 8388609.f;
-      key[i] = l[i] > -INFINITY ? (__float_as_uint(f) << Shift) + (base0 - i) : 0u;
+      for (int i = 0; i < EPL; ++i) {
+        const float f = scale == 0.f ? 8388609.f : fmaf(l[i] - lo, scale, 8388609.f);
+        key[i] = l[i] > -INFINITY ? (__float_as_uint(f) << Shift) + (base0 - i) : 0u;
+      }
+      sort_keys<EPL>(key);
     }
   }
-  sort_keys<EPL>(key);
+  uint32_t head = poison ? 0u : key[0];
   if (S.s.groups > 1) {
     uint32_t a, b;
     int level_tol = tol;
     if (level_scores) {
-      a = b = 0u;
+      a = sa;
+      b = sb;
       level_tol = static_cast<int>(4.f * (off * 8388592.f + 1.f)) + 1;
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        const uint32_t v = l[i] > -INFINITY ? __float_as_uint(fmaf(score[i], 8380000.f, 8388609.f)) & 0x7fffffu : 0u;
-        b = max(b, min(a, v));
-        a = max(a, v);
-      }
     } else {
-      a = key[0] >> Shift;
+      a = key[0] < Least ? 0u : key[0] >> Shift;
       b = S.s.group_top == 2 && EPL > 1 ? key[EPL > 1 ? 1 : 0] >> Shift : 0u;
       if (tol > 0 && S.s.group_top == 2) level_tol = 2 * tol;
     }
-    for (int o = S.lanes / 2; o > 0; o >>= 1) {
+    for (int o = 1 << S.lanes_log >> 1; o > 0; o >>= 1) {
       const uint32_t a2 = __shfl_xor_sync(kAll, a, o), b2 = __shfl_xor_sync(kAll, b, o);
       b = max(min(a, a2), max(b, b2));
       a = max(a, a2);
@@ -338,98 +448,173 @@ __device__ __forceinline__ void route_row(const RouteShape& S, const T* __restri
     const int zero = Bias ? B.zero : 1;
     const int level = a == 0u ? INT32_MIN : static_cast<int>(a) + (S.s.group_top == 1 ? 0 : b ? static_cast<int>(b) : zero);
     int better = 0;
+#pragma unroll 4
     for (int g = 0; g < S.s.groups; ++g) {
-      const int v = __shfl_sync(kAll, level, g * S.lanes);
+      const int v = __shfl_sync(kAll, level, g << S.lanes_log, L);
       better += v > level || (v == level && g < group);
     }
     const bool kept = group < S.s.groups && better < S.s.groups_kept;
-    const int least = __reduce_min_sync(kAll, kept ? level : INT32_MAX);
-    const int next = __reduce_max_sync(kAll, kept || group >= S.s.groups ? INT32_MIN : level);
+    const int least = ~row_max<L>(kept ? ~level : INT32_MIN);
+    const int next = row_max<L>(kept || group >= S.s.groups ? INT32_MIN : level);
     exact |= next > INT32_MIN && least - next <= level_tol;
-    if (!kept) {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) key[i] = 0u;
-    }
+    if (!kept) head = 0u;  // its list is never moved up
   }
-  uint32_t picked = 0u, after = 0u;  // lane j: the j-th key and the one after it
+  // Lists wait in shared memory, where moving up is one load; the long ones
+  // move through the registers. A list ends in a 0.
+  constexpr int Depth = list_depth(EPL);
+#pragma unroll
+  for (int i = 1; i < Depth - 1; ++i) list[i * 32] = key[i < EPL ? i : 0];
+  uint32_t picked = 0u, m = 0u;  // lane j: the j-th key
+  const uint32_t* next_key = list;
+#pragma unroll 3
   for (int j = 0; j <= k; ++j) {
-    const uint32_t m = __reduce_max_sync(kAll, key[0]);
+    m = row_max<L>(head);
     if (lane == j) picked = m;
-    if (lane == j - 1) after = m;
-    if (m == 0u) break;
-    if (key[0] == m) {
+    if (L == 32 && m < Least) break;
+    const bool up = head == m && (L == 32 || m >= Least);
+    if constexpr (Depth > 0) {
+      next_key += up ? 32 : 0;
+      if (up) head = *next_key;
+    } else if (up) {
 #pragma unroll
       for (int i = 0; i + 1 < EPL; ++i) key[i] = key[i + 1];
       key[EPL - 1] = 0u;
+      head = key[0];
     }
   }
-  if (lane >= k) picked = 0u;
+  uint32_t after = __shfl_down_sync(kAll, picked, 1);
+  if (lane == k - 1) after = m;  // the first one not chosen
+  if (lane >= k || picked < Least) picked = 0u;
+  if (after < Least) after = 0u;
   const auto expert = [&](uint32_t v) {
     const int slot = static_cast<int>((1u << Slots) - 1u - (v & ((1u << Slots) - 1u)));
     const int ln = slot / EPL;
-    return ln / S.lanes * S.per + (ln % S.lanes) * EPL + slot % EPL;
+    return (ln >> S.lanes_log) * S.per + (ln & ((1 << S.lanes_log) - 1)) * EPL + slot % EPL;
   };
   mine = picked ? expert(picked) : -1;
-  if (!Exact16 && picked && after && static_cast<int>((picked >> Shift) - (after >> Shift)) <= tol) {
-    const int other = expert(after);  // the same logit and bias: equal, and in order
-    const bool same = widen(row[mine]) == widen(row[other]) && (!Bias || bias[mine] == bias[other]);
-    exact |= !same;
+  // No lane takes a branch of its own up to here and below: the compiler
+  // guards every vote and shuffle behind one with a synchronisation of its
+  // own, which made half of this loop's instructions.
+  const bool near = !Exact16 && picked && after && static_cast<int>((picked >> Shift) - (after >> Shift)) <= tol;
+  if (!Exact16 && __any_sync(kAll, near)) {
+    // The pair's values themselves, in fp64: is the order right? At the last
+    // choice the one after the pair has to be further off.
+    const int a = near ? mine : 0, b = near ? expert(after) : 0;
+    double va = widen(row[a]), vb = widen(row[b]);
+    if constexpr (Bias) {
+      if (softmax) {
+        double all = 0;
+#pragma unroll 1
+        for (int e = lane; e < S.s.experts; e += L) {
+          const double v = widen(row[e]);
+          if (v > -INFINITY) all += exp(v - static_cast<double>(top));
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) all += __shfl_xor_sync(kAll, all, o);
+        va = exp(va - static_cast<double>(top)) / all;
+        vb = exp(vb - static_cast<double>(top)) / all;
+      } else {
+        va = 1.0 / (1.0 + exp(-va));
+        vb = 1.0 / (1.0 + exp(-vb));
+      }
+      va += static_cast<double>(bias[a]);
+      vb += static_cast<double>(bias[b]);
+    }
+    const uint32_t third = row_max<L>(head);  // the loop's last turn took `after` off its list
+    const bool crowded = lane == k - 1 && third >= Least && static_cast<int>((picked >> Shift) - (third >> Shift)) <= tol;
+    // A pair in the wrong order that is near no other is exchanged.
+    const bool wrong = near && !(va > vb || (va == vb && a < b));
+    const int near_before = __shfl_up_sync(kAll, near, 1, L), near_after = __shfl_down_sync(kAll, near, 1, L);
+    const int wrong_before = __shfl_up_sync(kAll, wrong, 1, L), before = __shfl_up_sync(kAll, a, 1, L);
+    const bool beside = (lane > 0 && near_before) || (lane < k - 1 && near_after);
+    exact |= (near && crowded) || (wrong && beside);
+    mine = wrong ? b : lane > 0 && lane < k && wrong_before ? before : mine;
   }
-  if (__any_sync(kAll, exact)) mine = choose_exact<T>(S, row, Bias ? bias : nullptr, EPL);
 
-  const float ml = mine >= 0 ? static_cast<float>(widen(row[mine])) : -INFINITY;
-  float w = 0.f;
+  const float chosen = static_cast<float>(widen(row[max(mine, 0)]));
+  const float ml = mine >= 0 ? chosen : -INFINITY;
+  float w;
   if (S.s.renormalise) {
-    // Shares of the chosen scores, from a common factor taken out of them:
-    // exp(l - m) under the softmax; under the sigmoid, where m <= 0,
-    // exp(l - m) / (1 + exp(l)) = sigmoid(l) * exp(-m).
-    float m = warp_max(ml);
-    if (!softmax) m = fminf(m, 0.f);
-    if (mine >= 0)
-      w = softmax ? expf(ml - m) : ml > 0.f ? 1.f / (1.f + expf(-ml)) : expf(ml - m) / (1.f + expf(ml));
-    const float all = warp_sum(w);
-    w = all > 0.f ? w / all : 0.f;
-  } else if (mine >= 0) {
+    // As chosen_share, in fp32.
+    float m = unordered(row_max<L>(ordered(ml)));
+    if (softmax) {
+      w = expf(ml - m);
+    } else {
+      const float e = ml > 0.f ? 1.f : expf(ml - fminf(m, 0.f));
+      w = __fdividef(e, 1.f + expf(-fabsf(ml)));
+    }
+    w = mine >= 0 ? w : 0.f;
+    const float all = row_sum<L>(w);
+    w = all > 0.f ? __fdividef(w, all) : 0.f;
+  } else {
     w = softmax ? expf(ml - top) / sum : 1.f / (1.f + expf(-ml));
+    w = mine >= 0 ? w : 0.f;
   }
-  weight = w * S.s.scale;
+  weight = poison ? NAN : w * S.s.scale;
+  return row_any<L>(exact && !poison);
 }
 
-// A block takes the tokens of a tile (all tiles in turn where no plan is made),
-// a warp one row at a time. With a plan it also leaves the tile's counts of
-// each expert, or, if the tile is all there is, the plan itself.
+// A block takes the tokens of a tile, 32 / L rows a warp at a time. With a plan
+// it also leaves the tile's counts of each expert, or, if the tile is all
+// there is, the plan itself.
 enum class PlanPart { None, Counts, Whole };
 
-template <typename T, int EPL, bool Bias>
-__global__ void __launch_bounds__(kRouteThreads)
+template <typename T, int L, int EPL, bool Bias>
+__global__ void __launch_bounds__(kRouteThreads, EPL > 8 ? 2 : 4)
     route_rows(RouteShape S, const T* __restrict__ logits, int64_t ld, bool whole, const float* __restrict__ bias,
                int tokens, int tile_tokens, int* __restrict__ indices, float* __restrict__ weights, PlanPart part,
                PlanView P) {
   extern __shared__ int shared[];  // chosen[tile_entries], then the plan's
-  __shared__ int sh[kPlanWarps];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k = S.s.k, E = S.s.experts;
-  BiasScale<EPL> B{};
-  if constexpr (Bias) {
-    const int group = lane / S.lanes, first = (lane % S.lanes) * EPL;
-    load_bias<EPL, value_bits(EPL)>(S, bias, group * S.per + first,
-                                    group < S.s.groups ? max(0, min(EPL, S.per - first)) : 0, B);
-  }
+  __shared__ int sh[kPlanWarps], doubtful;
+  __shared__ uint16_t doubts[kRouteRows];
+  __shared__ uint32_t lists[kRouteThreads / 32][list_depth(EPL) ? list_depth(EPL) * 32 : 1];
+  __shared__ __align__(16) float table[Bias ? L * bias_row(EPL) : 1];
+  constexpr int Rows = 32 / L;  // of a warp
+  const int lane = threadIdx.x & (L - 1), w = threadIdx.x >> 5, sub = (threadIdx.x & 31) / L, k = S.s.k, E = S.s.experts;
+  BiasScale B{};
+  if constexpr (Bias) B = load_bias<L, EPL>(S, bias, table);
+  if constexpr (list_depth(EPL) > 0) lists[w][(list_depth(EPL) - 1) * 32 + (threadIdx.x & 31)] = 0u;
   int* counts = shared + tile_tokens * k;
-  if (part == PlanPart::Counts) {
+  if (threadIdx.x == 0) doubtful = 0;
+  if (part == PlanPart::Counts)
     for (int e = threadIdx.x; e < P.stride; e += kRouteThreads) counts[e] = 0;
-    __syncthreads();
-  }
+  __syncthreads();
   const int t0 = blockIdx.x * tile_tokens, n = min(tile_tokens, tokens - t0);
-  for (int i = w; i < n; i += kRouteThreads / 32) {
-    const int64_t t = t0 + i;
+  // Every warp makes the same number of turns, so that the compiler knows the
+  // lanes to be together at each vote and shuffle (a loop it takes for
+  // divergent costs a synchronisation at each: 1.4x the instructions). Lanes
+  // past the last row do it again and keep it to themselves.
+  for (int i0 = 0; i0 < n; i0 += kRouteThreads / L) {
+    const int i = i0 + w * Rows;
+    const bool real = i + sub < n;
+    const int64_t t = t0 + (real ? i + sub : n - 1);
     int mine;
     float weight;
-    route_row<T, EPL, Bias>(S, logits + t * ld, whole, bias, B, mine, weight);
-    if (lane < k) {
+    const bool doubt =
+        route_row<T, L, EPL, Bias>(S, logits + t * ld, whole, bias, B, lists[w] + (threadIdx.x & 31), mine, weight);
+    if (lane == 0 && real && doubt) doubts[atomicAdd(&doubtful, 1)] = static_cast<uint16_t>(i + sub);
+    if (lane < k && real && !doubt) {
       indices[t * k + lane] = mine;
       weights[t * k + lane] = weight;
       if (part == PlanPart::Counts && mine >= 0) atomicAdd(&counts[mine], 1);
-      if (part == PlanPart::Whole) shared[i * k + lane] = mine;
+      if (part == PlanPart::Whole) shared[(i + sub) * k + lane] = mine;
+    }
+  }
+  // The rows in doubt, shared out among the warps.
+  __syncthreads();
+  if (doubtful > 0) {
+    RouteShape wide = S;
+    wide.lanes_log += L == 8 ? 2 : L == 16 ? 1 : 0;
+    for (int d = w; d < doubtful; d += kRouteThreads / 32) {
+      const int i = doubts[d], ln = threadIdx.x & 31;
+      const int64_t t = t0 + i;
+      float weight;
+      const int mine = route_exact<T, (EPL * L / 32 > 0 ? EPL * L / 32 : 1)>(wide, logits + t * ld, Bias ? bias : nullptr, weight);
+      if (ln >= k) continue;
+      indices[t * k + ln] = mine;
+      weights[t * k + ln] = weight;
+      if (part == PlanPart::Counts && mine >= 0) atomicAdd(&counts[mine], 1);
+      if (part == PlanPart::Whole) shared[i * k + ln] = mine;
     }
   }
   if (part == PlanPart::None) return;
@@ -438,7 +623,7 @@ __global__ void __launch_bounds__(kRouteThreads)
     for (int e = threadIdx.x; e < P.stride; e += kRouteThreads)
       P.counts[static_cast<int64_t>(blockIdx.x) * P.stride + e] = static_cast<uint16_t>(counts[e]);
   } else {
-    plan_alone<2>([&](int i) { return shared[i]; }, n * k, E, counts, counts + kPlanWarps * E, sh, P.offsets, P.order,
+    plan_alone<2>([&](int i) { return shared[i]; }, n * k, E, P.err, counts, counts + kPlanWarps * E, sh, P.offsets, P.order,
                   P.position);
   }
 }
@@ -452,8 +637,9 @@ __global__ void __launch_bounds__(kRouteThreads)
     route_grad_rows(spmvb_router_spec S, const T* __restrict__ logits, int64_t ld, int tokens,
                     const int* __restrict__ indices, const float* __restrict__ dweights, T* __restrict__ dlogits,
                     int64_t ldd, int* __restrict__ err) {
-  const int t = blockIdx.x * (kRouteThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (t >= tokens) return;
+  const int lane = threadIdx.x & 31, w0 = blockIdx.x * (kRouteThreads / 32) + (threadIdx.x >> 5);
+  const bool real = w0 < tokens;  // a warp past the last token repeats it and writes nothing
+  const int64_t t = real ? w0 : tokens - 1;
   const int E = S.experts, k = S.k;
   const T* row = logits + t * ld;
   int e = -1;
@@ -524,22 +710,32 @@ __global__ void __launch_bounds__(kRouteThreads)
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     const int x = lane * EPL + i;
-    if (x < E) dlogits[t * ldd + x] = narrow<T, float>(poison ? NAN : g[i]);
+    if (x < E && real) dlogits[t * ldd + x] = narrow<T, float>(poison ? NAN : g[i]);
   }
 }
 
-// Lanes of a group: the warp shared out among the groups, a power of two each.
-int lanes_per_group(const spmvb_router_spec& s) {
-  int lanes = 32;
-  while (lanes * s.groups > 32) lanes /= 2;
-  return lanes;
+// Lanes of a group: the row's lanes shared out among the groups, a power of
+// two each.
+int lanes_per_group(const spmvb_router_spec& s, int lanes) {
+  int n = lanes;
+  while (n * s.groups > lanes) n /= 2;
+  return n;
 }
 // Experts of a lane, rounded up to a power of two: at most 64, as of 1,020
 // experts in 17 groups.
-int slots_per_lane(const spmvb_router_spec& s) {
+int slots_per_lane(const spmvb_router_spec& s, int lanes) {
   int slots = 1;
-  while (slots * lanes_per_group(s) < s.experts / s.groups) slots *= 2;
+  while (slots * lanes_per_group(s, lanes) < s.experts / s.groups) slots *= 2;
   return slots;
+}
+
+// Lanes of a row: as few as leave a lane eight experts, where the lanes can
+// hold the choices and the groups and there are rows to fill the GPU.
+int row_lanes(const spmvb_router_spec& s, int tokens, int sm_count) {
+  if (tokens <= sm_count * 8) return 32;
+  int lanes = 8;
+  while (lanes < 32 && (lanes * 8 < s.experts || lanes < s.k || lanes < s.groups)) lanes *= 2;
+  return (s.groups & (s.groups - 1)) == 0 ? lanes : 32;
 }
 
 int slots_for(int experts) {
@@ -712,19 +908,25 @@ spmvb_status spmvb_router_route(spmvb_router R, spmvb_dtype dtype, int32_t token
                         : tokens <= tile ? PlanPart::Whole
                         : plan_is_one_block(P) ? PlanPart::None : PlanPart::Counts;
   if (tokens > 0) {
-    SPMVB_TRY(with_logits(dtype, slots_per_lane(S), [&](auto tv, auto epl) -> spmvb_status {
+    const int L = row_lanes(S, tokens, R->ctx->sm_count);
+    SPMVB_TRY(with_logits(dtype, slots_per_lane(S, L), [&](auto tv, auto epl) -> spmvb_status {
       using T = decltype(tv);
       constexpr int EPL = decltype(epl)::value;
-      const RouteShape shape{S, S.experts / S.groups, lanes_per_group(S)};
+      const RouteShape shape{S, S.experts / S.groups, __builtin_ctz(lanes_per_group(S, L))};
       const int vb = std::min<int>(16, EPL * sizeof(T));
-      const bool whole = S.experts == 32 * EPL && access_bytes(sizeof(T), {{d_logits, ld_logits}}, vb / sizeof(T)) == vb;
-      // Without a plan a block takes a row a warp where that many blocks have room.
-      const int rows = part == PlanPart::None ? std::max(kRouteThreads / 32, static_cast<int>(ceil_div(tokens, int64_t(R->ctx->sm_count) * 4)))
-                                              : tile;
+      const bool whole = S.experts == L * EPL && access_bytes(sizeof(T), {{d_logits, ld_logits}}, vb / sizeof(T)) == vb;
+      // Without a plan a block takes one row a lane group where that many blocks have room.
+      const int at_once = kRouteThreads / L;
+      const int rows = part != PlanPart::None ? tile
+                                              : std::min(kRouteRows, static_cast<int>(ceil_div(ceil_div(tokens, int64_t(R->ctx->sm_count) * 4), at_once)) * at_once);
       const size_t shared = part == PlanPart::None     ? 0
                             : part == PlanPart::Counts ? (static_cast<size_t>(rows) * S.k + P.stride) * 4
                                                        : (static_cast<size_t>(rows) * S.k + (kPlanWarps + 1) * S.experts) * 4;
-      const auto kernel = d_bias ? route_rows<T, EPL, true> : route_rows<T, EPL, false>;
+      auto kernel = d_bias ? route_rows<T, 32, EPL, true> : route_rows<T, 32, EPL, false>;
+      if constexpr (EPL <= 8) {
+        if (L == 16) kernel = d_bias ? route_rows<T, 16, EPL, true> : route_rows<T, 16, EPL, false>;
+        if (L == 8) kernel = d_bias ? route_rows<T, 8, EPL, true> : route_rows<T, 8, EPL, false>;
+      }
       kernel<<<static_cast<int>(ceil_div(tokens, rows)), kRouteThreads, shared, s>>>(
           shape, static_cast<const T*>(d_logits), ld_logits, whole, d_bias, tokens, rows, d_indices, d_weights, part, P);
       count_launch();
