@@ -1,25 +1,49 @@
 // The transposed product of a selection: the stable order of the tokens by the
 // row they name, and the embedding gradient made with it.
 //
-// Order. The entries are sorted by key (the row named, or n for none) with a
-// least-significant-digit radix sort, kDigitBits at a time. One pass: every
-// tile of kTile entries counts its digits (digit_counts); one warp per digit
-// turns the counts of all tiles into running sums (digit_scan); every tile
-// ranks its entries among the equal digits before them and writes them to
-// their places (digit_scatter). Ranks follow the entries' order, so the sort
-// is stable and nothing depends on timing.
+// Order, by the number of tokens:
+//   up to kSelfTokens   every block of the gradient ranks all tokens itself: a
+//                       token's place is the number of smaller (row, token)
+//                       pairs, 0.5 us of comparisons against a launch of 2.5
+//   up to kRankTokens   the same ranks, by a kernel of one block per 64 tokens
+//   up to kBlockTokens  least-significant-digit radix sort by one block, in
+//                       shared memory
+//   more                the same by many: every tile of kTile tokens counts its
+//                       digits (digit_counts), then ranks its tokens among the
+//                       equal digits before them and writes them to their
+//                       places (digit_scatter), which adds up the tiles'
+//                       counts itself up to kOwnTiles tiles and has them
+//                       summed by digit_scan beyond.
+// Ranks follow the tokens' order, so the order is stable and nothing depends
+// on timing.
 //
 // Gradient. dtable[r] = scale * sum of dout[t] over the tokens that name r:
 // in sorted order the tokens of one row are neighbours (a run). A block takes
-// kChunk sorted entries and a range of columns, adds each run in registers
-// and writes the runs that lie inside its chunk. A run that crosses a chunk's
-// edge leaves its part in scratch (slot 0: the run came in from the chunk
-// before, slot 1: it begins here and goes on), and the chunk where it begins
-// adds the parts in chunk order afterwards (join_runs). A frequent token is so
-// spread over many blocks, in a fixed order of summation.
+// chunks of kChunk sorted tokens and a range of columns, adds each run in
+// registers and writes the runs that lie inside a chunk. A run that crosses a
+// chunk's edge leaves its part in scratch (slot 0: the run came in from the
+// chunk before, slot 1: it begins here and goes on); the last of its blocks to
+// arrive adds the parts in chunk order. A frequent token is so spread over
+// many blocks, in a fixed order of summation. Where the gradient is not added
+// to what is there, the rows that no token names are written as well
+// (empty_rows), in the launch that sorts: its other blocks find the rows named
+// in their range by reading all tokens, so the sort takes no time of its own.
+// The table is written once, and that bounds the kernels (1.07 GB of 1.2 GB
+// for 16,384 tokens of 4,096 bf16 values and 131,072 rows).
 #include "select.cuh"
 
 namespace spmvb {
+
+// Scratch of the sort for a number of tokens.
+struct SortSpace {
+  DevBuf keys[2], vals[2], counts, totals;
+  spmvb_status alloc(int64_t tokens);
+};
+struct Sorted {
+  const uint32_t* keys;  // ascending; the number of rows for tokens that select nothing
+  const int* entries;    // in token order among equal keys
+};
+
 namespace {
 
 constexpr int kDigitBits = 9;
@@ -28,32 +52,35 @@ constexpr int kSortThreads = 256;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kPerThread = 4;
 constexpr int kTile = kSortThreads * kPerThread;
+constexpr int kOwnTiles = 64;
+constexpr int kSelfTokens = 256;
+constexpr int kRankTokens = 2048;
+constexpr int kBlockTokens = 16384;
+constexpr int kOrderThreads = 1024;
 
+// The key of an index that has been loaded. The report comes after all loads
+// of a thread: its store would hold the next one back.
 __device__ __forceinline__ uint32_t key_of(int i, uint32_t n, int* err) {
   if (i >= 0 && static_cast<uint32_t>(i) >= n) *err = 1;
   return i < 0 || static_cast<uint32_t>(i) >= n ? n : static_cast<uint32_t>(i);
 }
 
-// Keys of a pass: the indices themselves (First) or the last pass's keys.
-template <bool First>
-__device__ __forceinline__ uint32_t load_key(const void* src, int64_t i, uint32_t n, int* err) {
-  if (First) return key_of(static_cast<const int*>(src)[i], n, err);
-  return static_cast<const uint32_t*>(src)[i];
-}
-
 // counts[digit * tiles + tile].
 template <bool First>
 __global__ void __launch_bounds__(kSortThreads)
-    digit_counts(const void* __restrict__ src, int64_t count, uint32_t n, int shift, int tiles, int* __restrict__ counts,
+    digit_counts(const int* __restrict__ src, int64_t count, uint32_t n, int shift, int tiles, int* __restrict__ counts,
                  int* __restrict__ err) {
   __shared__ int c[kDigits];
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) c[d] = 0;
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kTile + threadIdx.x;
+  int raw[kPerThread];
+#pragma unroll
+  for (int q = 0; q < kPerThread; ++q) raw[q] = i0 + q * kSortThreads < count ? __ldg(src + i0 + q * kSortThreads) : -1;
   __syncthreads();
-  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kTile;
 #pragma unroll
   for (int q = 0; q < kPerThread; ++q) {
-    const int64_t i = i0 + q * kSortThreads + threadIdx.x;
-    if (i < count) atomicAdd(&c[(load_key<First>(src, i, n, err) >> shift) & (kDigits - 1)], 1);
+    const uint32_t key = First ? key_of(raw[q], n, err) : static_cast<uint32_t>(raw[q]);
+    if (i0 + q * kSortThreads < count) atomicAdd(&c[(key >> shift) & (kDigits - 1)], 1);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) counts[static_cast<int64_t>(d) * tiles + blockIdx.x] = c[d];
@@ -105,41 +132,75 @@ static_assert(kDigits == 2 * kSortThreads);
 
 template <bool First>
 __global__ void __launch_bounds__(kSortThreads)
-    digit_scatter(const void* __restrict__ src, const int* __restrict__ src_vals, int64_t count, uint32_t n, int shift,
-                  int tiles, const int* __restrict__ counts, const int* __restrict__ totals,
+    digit_scatter(const int* __restrict__ src, const int* __restrict__ src_vals, int64_t count, uint32_t n, int shift,
+                  int tiles, bool scanned, const int* __restrict__ counts, const int* __restrict__ totals,
                   uint32_t* __restrict__ dst_keys, int* __restrict__ dst_vals, int* __restrict__ err) {
   __shared__ int wc[kSortWarps][kDigits];  // a warp's count of each digit, then its first place
   __shared__ int sh[kSortWarps];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   for (int d = threadIdx.x; d < kSortWarps * kDigits; d += kSortThreads) (&wc[0][0])[d] = 0;
-  __syncthreads();
   // A warp's entries are neighbours: 32 * kPerThread of them, in rounds of 32.
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kTile + w * (32 * kPerThread) + lane;
-  uint32_t key[kPerThread];
-  int rank[kPerThread];
+  int raw[kPerThread], val[kPerThread];
 #pragma unroll
   for (int q = 0; q < kPerThread; ++q) {
     const int64_t i = i0 + q * 32;
-    const bool in = i < count;
-    key[q] = in ? load_key<First>(src, i, n, err) : 0u;
-    const int d = in ? static_cast<int>((key[q] >> shift) & (kDigits - 1)) : kDigits + lane;
-    const unsigned same = __match_any_sync(0xffffffffu, d);
-    const unsigned before = same & ((1u << lane) - 1u);
-    const int base = in ? wc[w][d] : 0;
+    raw[q] = i < count ? __ldg(src + i) : -1;
+    val[q] = First ? static_cast<int>(i) : i < count ? __ldg(src_vals + i) : 0;
+  }
+  // The digit's entries in the tiles before, and in all.
+  int v[2], at_tile[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t row = static_cast<int64_t>(2 * threadIdx.x + h) * tiles;
+    if (scanned) {
+      v[h] = totals[2 * threadIdx.x + h];
+      at_tile[h] = counts[row + blockIdx.x];
+    } else {
+      v[h] = at_tile[h] = 0;
+#pragma unroll 8
+      for (int t = 0; t < tiles; ++t) {
+        const int c = __ldg(counts + row + t);
+        v[h] += c;
+        at_tile[h] += t < static_cast<int>(blockIdx.x) ? c : 0;
+      }
+    }
+  }
+  __syncthreads();
+  uint32_t key[kPerThread];
+  int rank[kPerThread];
+  unsigned same[kPerThread];
+#pragma unroll
+  for (int q = 0; q < kPerThread; ++q) {
+    key[q] = First ? key_of(raw[q], n, err) : static_cast<uint32_t>(raw[q]);
+    // The lanes with the same digit, from one vote a bit.
+    same[q] = __ballot_sync(0xffffffffu, i0 + q * 32 < count);
+#pragma unroll
+    for (int bit = 0; bit < kDigitBits; ++bit) {
+      const bool on = key[q] >> (shift + bit) & 1u;
+      const unsigned vote = __ballot_sync(0xffffffffu, on);
+      same[q] &= on ? vote : ~vote;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kPerThread; ++q) {
+    const bool in = i0 + q * 32 < count;
+    const int d = static_cast<int>((key[q] >> shift) & (kDigits - 1));
+    const unsigned before = same[q] & ((1u << lane) - 1u);
+    const int base = wc[w][d];
     rank[q] = base + __popc(before);
     __syncwarp();
-    if (in && before == 0) wc[w][d] = base + __popc(same);
+    if (in && before == 0) wc[w][d] = base + __popc(same[q]);
     __syncwarp();
   }
   __syncthreads();
   // First place of each digit: all smaller digits, then this digit in the
   // tiles and the warps before.
-  int v[2] = {totals[2 * threadIdx.x], totals[2 * threadIdx.x + 1]};
   scan_digits(v, sh);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int d = 2 * threadIdx.x + h;
-    int at = v[h] + counts[static_cast<int64_t>(d) * tiles + blockIdx.x];
+    int at = v[h] + at_tile[h];
 #pragma unroll
     for (int i = 0; i < kSortWarps; ++i) {
       const int c = wc[i][d];
@@ -150,85 +211,437 @@ __global__ void __launch_bounds__(kSortThreads)
   __syncthreads();
 #pragma unroll
   for (int q = 0; q < kPerThread; ++q) {
-    const int64_t i = i0 + q * 32;
-    if (i >= count) continue;
+    if (i0 + q * 32 >= count) continue;
     const int at = wc[w][(key[q] >> shift) & (kDigits - 1)] + rank[q];
     dst_keys[at] = key[q];
-    dst_vals[at] = First ? static_cast<int>(i) : src_vals[i];
+    dst_vals[at] = val[q];
+  }
+}
+
+// Place of a (row, token) pair, as one word, among all `count` (padded with
+// ones to a multiple of 4): the smaller ones. `each` threads, a power of two
+// of neighbours, share the count; all of them get it.
+__device__ __forceinline__ int rank_among(uint32_t mine, const uint32_t* pairs, int count, int each, int part) {
+  int below = 0;
+  const uint4* p = reinterpret_cast<const uint4*>(pairs);
+#pragma unroll 4
+  for (int i = part; i < (count + 3) / 4; i += each) {
+    const uint4 v = p[i];
+    below += (v.x < mine) + (v.y < mine) + (v.z < mine) + (v.w < mine);
+  }
+  for (int off = each / 2; off > 0; off >>= 1) below += __shfl_xor_sync(0xffffffffu, below, off);
+  return below;
+}
+
+// Sorted keys and tokens by counting: 64 tokens a block, 4 threads a token.
+__global__ void __launch_bounds__(256)
+    rank_tokens(const int* __restrict__ src, int count, uint32_t n, int token_bits, uint32_t* __restrict__ keys,
+                int* __restrict__ vals, int* __restrict__ err) {
+  __shared__ __align__(16) uint32_t pairs[kRankTokens];
+  const int padded = (count + 3) / 4 * 4;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < padded; i += 256) {
+    const int raw = i < count ? __ldg(src + i) : -1;
+    const uint32_t key = raw < 0 || static_cast<uint32_t>(raw) >= n ? n : static_cast<uint32_t>(raw);
+    pairs[i] = i < count ? key << token_bits | static_cast<uint32_t>(i) : 0xffffffffu;
+  }
+  __syncthreads();
+  const int i = blockIdx.x * 64 + (threadIdx.x >> 2);
+  const int at = rank_among(pairs[min(i, count - 1)], pairs, count, 4, threadIdx.x & 3);
+  if (i < count && (threadIdx.x & 3) == 0) {
+    keys[at] = pairs[i] >> token_bits;
+    vals[at] = i;
+    key_of(__ldg(src + i), n, err);  // reports an index past the end
   }
 }
 
 // ---- embedding gradient ----------------------------------------------------------
-constexpr int kChunk = 16;
 constexpr int kGradThreads = 256;
+constexpr int kMinAcross = 8;  // threads along a row, at least
 
-template <typename T, typename G, int N>
-__device__ __forceinline__ void store_row(G* dst, const typename AccOf<T>::type (&sum)[N],
-                                          typename AccOf<T>::type scale, bool accumulate) {
-  using Acc = typename AccOf<T>::type;
+// N values of a row, by accesses of up to 16 bytes; the row is aligned to them.
+template <typename G, int N>
+struct RowPack {
+  static constexpr int VB = N * sizeof(G) > 16 ? 16 : N * static_cast<int>(sizeof(G));
+  static constexpr int M = VB / static_cast<int>(sizeof(G));
+  Pack<G, VB> p[N / M];
+  __device__ __forceinline__ void load(const G* src) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    Acc v = sum[i] * scale;
-    if (accumulate) v += widen(dst[i]);
-    dst[i] = narrow<G, Acc>(v);
+    for (int i = 0; i < N / M; ++i) p[i] = ld_pack_stream<G, VB>(src + i * M);
   }
-}
+  __device__ __forceinline__ void store(G* dst) const {
+#pragma unroll
+    for (int i = 0; i < N / M; ++i) st_pack_stream<G, VB>(dst + i * M, p[i]);
+  }
+};
 
-template <typename T, typename G, int VB>
-__global__ void __launch_bounds__(kGradThreads)
-    run_sums(const uint32_t* __restrict__ keys, const int* __restrict__ vals, int64_t count, uint32_t n,
-             const T* __restrict__ dout, int64_t ldo, typename AccOf<T>::type scale, G* __restrict__ dtable, int64_t ldt,
-             int packs, int width, bool accumulate, typename AccOf<T>::type* __restrict__ parts) {
-  using Acc = typename AccOf<T>::type;
-  constexpr int N = Pack<T, VB>::N;
-  const int v = blockIdx.y * kGradThreads + threadIdx.x;
-  if (v >= packs) return;
-  const int64_t c = static_cast<int64_t>(v) * N;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kChunk;
-  const int64_t last = min(first + kChunk, count);
-  const bool came_in = first > 0 && keys[first - 1] == keys[first];
-  const bool goes_on = last < count && keys[last] == keys[last - 1];
-  Acc sum[N] = {};
-  int64_t begin = first;
-  for (int64_t i = first; i < last; ++i) {
-    const uint32_t key = keys[i];
-    if (key >= n) return;  // the entries that select nothing come last
-    const Pack<T, VB> p = ld_pack_stream<T, VB>(dout + vals[i] * ldo + c);
-#pragma unroll
-    for (int q = 0; q < N; ++q) sum[q] += widen(p.v[q]);
-    if (i + 1 < last && keys[i + 1] == key) continue;
-    const bool in = begin == first && came_in, on = i + 1 == last && goes_on;
-    if (in || on) {
-      Acc* part = parts + (static_cast<int64_t>(blockIdx.x) * 2 + (in ? 0 : 1)) * width + c;
-#pragma unroll
-      for (int q = 0; q < N; ++q) part[q] = sum[q];
+struct EmptyRows {
+  char* table;           // null: nothing to write
+  int64_t pitch, bytes;  // of a row
+  int rows, per_block;   // rows of a block
+  bool wide;             // 16 bytes at a time, else `elem`
+  int elem;
+};
+
+// The rows of one block's range that no token names, a warp a row. `named`: a
+// bit per row of the range.
+__device__ __forceinline__ void empty_rows(const EmptyRows& Z, int block, const int* __restrict__ tokens, int count,
+                                           uint32_t* named) {
+  const int r0 = block * Z.per_block, r1 = min(r0 + Z.per_block, Z.rows), lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < (Z.per_block + 31) / 32; i += blockDim.x) named[i] = 0u;
+  __syncthreads();
+#pragma unroll 4
+  for (int i = threadIdx.x; i < count; i += blockDim.x) {
+    const int r = __ldg(tokens + i);
+    if (r >= r0 && r < r1) atomicOr(&named[(r - r0) >> 5], 1u << ((r - r0) & 31));
+  }
+  __syncthreads();
+  const int warps = blockDim.x >> 5;
+  for (int r = r0 + (threadIdx.x >> 5); r < r1; r += warps) {
+    if (named[(r - r0) >> 5] >> ((r - r0) & 31) & 1u) continue;
+    char* row = Z.table + r * Z.pitch;
+    if (Z.wide) {
+#pragma unroll 4
+      for (int64_t i = lane; i < Z.bytes / 16; i += 32) __stcs(reinterpret_cast<uint4*>(row) + i, make_uint4(0, 0, 0, 0));
+    } else if (Z.elem == 2) {
+#pragma unroll 4
+      for (int64_t i = lane; i < Z.bytes / 2; i += 32) __stcs(reinterpret_cast<uint16_t*>(row) + i, uint16_t(0));
     } else {
-      store_row<T, G, N>(dtable + key * ldt + c, sum, scale, accumulate);
+#pragma unroll 4
+      for (int64_t i = lane; i < Z.bytes / 4; i += 32) __stcs(reinterpret_cast<uint32_t*>(row) + i, 0u);
     }
+  }
+}
+constexpr int kMaxEmptyRows = 8192;  // of a block: 1 KB of bits
+
+// Block 0 sorts up to kBlockTokens tokens; the others write the empty rows.
+// Shared memory: keys, 16-bit tokens, 16-bit counts per warp and digit.
+constexpr size_t kOrderShared = kBlockTokens * 6 + (kOrderThreads / 32) * kDigits * 2;
+__global__ void __launch_bounds__(kOrderThreads)
+    order_tokens(const int* __restrict__ src, int count, uint32_t n, int bits, uint32_t* __restrict__ keys,
+                 int* __restrict__ vals, EmptyRows Z, int* __restrict__ err) {
+  extern __shared__ __align__(16) uint32_t shared[];
+  if (blockIdx.x > 0) {
+    empty_rows(Z, blockIdx.x - 1, src, count, shared);
+    return;
+  }
+  constexpr int Warps = kOrderThreads / 32, Rounds = kBlockTokens / kOrderThreads;
+  uint32_t* sk = shared;
+  uint16_t* sv = reinterpret_cast<uint16_t*>(shared + kBlockTokens);
+  uint16_t* wc = sv + kBlockTokens;
+  __shared__ int sh[kDigits / 32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int rounds = (count + kOrderThreads - 1) / kOrderThreads;  // of 32 tokens a warp, neighbours
+  const int i0 = w * rounds * 32 + lane;
+  uint32_t key[Rounds], place[Rounds];  // place: token << 16 | rank
 #pragma unroll
-    for (int q = 0; q < N; ++q) sum[q] = 0;
-    begin = i + 1;
+  for (int q = 0; q < Rounds; ++q)
+    key[q] = q < rounds && i0 + q * 32 < count ? static_cast<uint32_t>(__ldg(src + i0 + q * 32)) : 0u;
+#pragma unroll
+  for (int q = 0; q < Rounds; ++q) {
+    key[q] = key_of(static_cast<int>(key[q]), n, err);
+    place[q] = static_cast<uint32_t>(i0 + q * 32) << 16;
+  }
+  for (int shift = 0; shift < bits; shift += kDigitBits) {
+    uint32_t* zero = reinterpret_cast<uint32_t*>(wc);
+    for (int i = threadIdx.x; i < Warps * kDigits / 2; i += kOrderThreads) zero[i] = 0u;
+    __syncthreads();
+    if (shift > 0) {
+#pragma unroll
+      for (int q = 0; q < Rounds; ++q)
+        if (q < rounds && i0 + q * 32 < count) {
+          key[q] = sk[i0 + q * 32];
+          place[q] = static_cast<uint32_t>(sv[i0 + q * 32]) << 16;
+        }
+    }
+    uint16_t* mine = wc + w * kDigits;
+#pragma unroll
+    for (int q = 0; q < Rounds; ++q) {
+      if (q >= rounds) break;
+      // The lanes with the same digit, from one vote a bit.
+      const bool in = i0 + q * 32 < count;
+      unsigned same = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+      for (int bit = 0; bit < kDigitBits; ++bit) {
+        const bool on = key[q] >> (shift + bit) & 1u;
+        const unsigned vote = __ballot_sync(0xffffffffu, on);
+        same &= on ? vote : ~vote;
+      }
+      const int d = static_cast<int>((key[q] >> shift) & (kDigits - 1));
+      const unsigned before = same & ((1u << lane) - 1u);
+      const int base = mine[d];
+      __syncwarp();
+      if (in && before == 0) mine[d] = static_cast<uint16_t>(base + __popc(same));
+      place[q] = (place[q] & 0xffff0000u) | static_cast<uint32_t>(base + __popc(before));
+      __syncwarp();
+    }
+    __syncthreads();
+    // First place of each digit and warp.
+    int all = 0, incl = 0;
+    const int d = threadIdx.x;
+    if (d < kDigits) {
+#pragma unroll 8
+      for (int i = 0; i < Warps; ++i) all += wc[i * kDigits + d];
+      incl = all;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += u;
+      }
+      if (lane == 31) sh[w] = incl;
+    }
+    __syncthreads();
+    if (d < kDigits) {
+      int at = incl - all;
+      for (int i = 0; i < w; ++i) at += sh[i];
+#pragma unroll 8
+      for (int i = 0; i < Warps; ++i) {
+        const int c = wc[i * kDigits + d];
+        wc[i * kDigits + d] = static_cast<uint16_t>(at);
+        at += c;
+      }
+    }
+    __syncthreads();
+    const bool last = shift + kDigitBits >= bits;
+#pragma unroll
+    for (int q = 0; q < Rounds; ++q) {
+      if (q >= rounds || i0 + q * 32 >= count) continue;
+      const int at = mine[(key[q] >> shift) & (kDigits - 1)] + static_cast<int>(place[q] & 0xffffu);
+      if (last) {
+        keys[at] = key[q];
+        vals[at] = static_cast<int>(place[q] >> 16);
+      } else {
+        sk[at] = key[q];
+        sv[at] = static_cast<uint16_t>(place[q] >> 16);
+      }
+    }
+    __syncthreads();
   }
 }
 
-// Adds the parts of the run that begins in this chunk and goes on.
-template <typename T, typename G>
+__global__ void __launch_bounds__(256) write_empty_rows(const int* __restrict__ src, int count, EmptyRows Z) {
+  __shared__ uint32_t named[kMaxEmptyRows / 32];
+  empty_rows(Z, blockIdx.x, src, count, named);
+}
+
+struct GradView {
+  const uint32_t* keys;  // sorted (unless the block sorts)
+  const int* vals;
+  const int* tokens;
+  int count;
+  uint32_t rows;
+  int chunks, chunk_blocks;  // blocks of the grid's x that take chunks; the others write empty rows
+  int width, packs, across;  // columns, packs of them, threads along a row
+  int64_t ldo, ldt;
+  void* parts;
+  unsigned* tickets;  // chunks x gridDim.y, all 0 between calls
+  EmptyRows empty;    // where the block sorts
+  int* err;
+};
+
+// Chunks from `from` on, in steps of `dir`, whose edge towards it continues
+// the run of `key`: steps that double, then halve.
+template <int Chunk>
+__device__ __forceinline__ int run_reach(const uint32_t* keys, int count, uint32_t key, int from, int dir) {
+  const auto on = [&](int steps) {  // does the run still hold `steps` chunks on?
+    const int64_t q = from + static_cast<int64_t>(dir) * steps;
+    const int64_t i = dir > 0 ? q * Chunk : (q + 1) * Chunk - 1;
+    return q >= 0 && i < count && keys[i] == key;
+  };
+  int have = 0, step = 1;
+  while (on(have + step)) {
+    have += step;
+    step *= 2;
+  }
+  for (step /= 2; step > 0; step /= 2)
+    if (on(have + step)) have += step;
+  return have;
+}
+
+// Tokens of a chunk: few where there are few, to spread them.
+constexpr int chunk_of(bool self) { return self ? 4 : 16; }
+// Packs of a thread, `across` packs apart: 16 bytes in all, 4 packs at most.
+constexpr int packs_of(int bytes) { return bytes >= 16 ? 1 : 16 / bytes > 4 ? 4 : 16 / bytes; }
+
+template <typename T, typename G, int N, bool Self, bool Add>
 __global__ void __launch_bounds__(kGradThreads)
-    join_runs(const uint32_t* __restrict__ keys, int64_t count, uint32_t n, typename AccOf<T>::type scale,
-              G* __restrict__ dtable, int64_t ldt, int width, bool accumulate,
-              const typename AccOf<T>::type* __restrict__ parts) {
+    grad_rows(GradView A, const T* __restrict__ dout, typename AccOf<T>::type scale, G* __restrict__ dtable) {
   using Acc = typename AccOf<T>::type;
-  const int64_t chunk = blockIdx.x, first = chunk * kChunk, last = min(first + kChunk, count);
-  if (last >= count) return;
-  const uint32_t key = keys[last - 1];
-  if (key >= n || keys[last] != key) return;                             // nothing goes on
-  if (keys[first] == key && first > 0 && keys[first - 1] == key) return;  // it began before
-  const int c = blockIdx.y * kGradThreads + threadIdx.x;
-  if (c >= width) return;
-  Acc sum = parts[(chunk * 2 + 1) * width + c];
-  for (int64_t q = chunk + 1; q * kChunk < count && keys[q * kChunk] == key; ++q) sum += parts[q * 2 * width + c];
-  const Acc one[1] = {sum};
-  store_row<T, G, 1>(dtable + key * ldt + c, one, scale, accumulate);
+  constexpr int VB = N * sizeof(T), M = packs_of(VB);
+  constexpr int Chunk = chunk_of(Self);
+  constexpr int Batch = Self || Add ? 4 : 8;  // rows loaded before the first is added
+  __shared__ __align__(16) uint32_t pairs[Self ? kSelfTokens : 4];
+  __shared__ uint32_t self_keys[Self ? kSelfTokens : 1];
+  __shared__ int self_vals[Self ? kSelfTokens : 1];
+  const uint32_t* keys = A.keys;
+  const int* vals = A.vals;
+  if constexpr (Self) {
+    if (static_cast<int>(blockIdx.x) >= A.chunk_blocks) {
+      empty_rows(A.empty, blockIdx.x - A.chunk_blocks, A.tokens, A.count, self_keys);
+      return;
+    }
+    // Rows have at most 23 bits, tokens 8.
+    const int padded = (A.count + 3) / 4 * 4;
+    for (int i = threadIdx.x; i < padded; i += kGradThreads)
+      pairs[i] = i < A.count ? key_of(__ldg(A.tokens + i), A.rows, A.err) << 8 | static_cast<uint32_t>(i) : 0xffffffffu;
+    __syncthreads();
+    int each = 1;  // threads of a token
+    while (each < 32 && A.count * each * 2 <= kGradThreads) each *= 2;
+    const int i = threadIdx.x / each;
+    const int at = rank_among(pairs[min(i, A.count - 1)], pairs, A.count, each, threadIdx.x % each);
+    if (i < A.count && threadIdx.x % each == 0) {
+      self_keys[at] = pairs[i] >> 8;
+      self_vals[at] = i;
+    }
+    __syncthreads();
+    keys = self_keys;
+    vals = self_vals;
+  }
+
+  // A chunk's keys with the one before and the one after it, and its tokens.
+  constexpr int Span = Chunk + 2;
+  constexpr int MaxDown = kGradThreads / kMinAcross;
+  __shared__ uint32_t ck[MaxDown * Span];
+  __shared__ int cv[MaxDown * Span];
+  __shared__ int joined[MaxDown][2][2];  // by slot: first and last chunk of a run whose parts are all there
+  const int down = kGradThreads / A.across;
+  const int x = threadIdx.x % A.across, y = threadIdx.x / A.across;
+  for (int i = threadIdx.x; i < down * Span; i += kGradThreads) {
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) * down + i / Span) * Chunk + i % Span - 1;
+    const bool in = at >= 0 && at < A.count;
+    ck[i] = in ? keys[at] : 0xffffffffu;
+    cv[i] = in ? vals[at] : 0;
+  }
+  __syncthreads();
+  const int chunk = blockIdx.x * down + y, v0 = blockIdx.y * A.across * M + x;
+  const uint32_t* k = ck + y * Span + 1;
+  const int* t = cv + y * Span + 1;
+  Acc* parts = static_cast<Acc*>(A.parts);
+  const bool mine = chunk < A.chunks;
+  // Entries that select nothing (key = rows) come last; past the end it is ~0.
+  const bool came_in = k[0] < A.rows && k[-1] == k[0];
+  const bool goes_on = k[Chunk - 1] < A.rows && k[Chunk] == k[Chunk - 1];
+  bool in_first = came_in;
+  const auto ends = [&](int i) { return i == Chunk - 1 || k[i + 1] != k[i]; };
+  if (mine) {
+    Acc sum[M][N] = {};
+#pragma unroll
+    for (int b = 0; b < Chunk; b += Batch) {
+      Pack<T, VB> p[Batch][M];
+      RowPack<G, N> old[Add ? Batch : 1][M];
+#pragma unroll
+      for (int q = 0; q < Batch; ++q) {
+        if (k[b + q] >= A.rows) continue;
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const int v = v0 + m * A.across;
+          if (v >= A.packs) continue;
+          p[q][m] = ld_pack_stream<T, VB>(dout + t[b + q] * A.ldo + static_cast<int64_t>(v) * N);
+          if (Add && ends(b + q)) old[Add ? q : 0][m].load(dtable + k[b + q] * A.ldt + static_cast<int64_t>(v) * N);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < Batch; ++q) {
+        const uint32_t key = k[b + q];
+        if (key >= A.rows) continue;
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int i = 0; i < N; ++i) sum[m][i] += widen(p[q][m].v[i]);
+        if (!ends(b + q)) continue;
+        const bool part = in_first || (b + q == Chunk - 1 && goes_on);
+        Acc* to = parts + (static_cast<int64_t>(chunk) * 2 + (in_first ? 0 : 1)) * A.width;
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const int v = v0 + m * A.across;
+          if (v >= A.packs) continue;
+          const int64_t c = static_cast<int64_t>(v) * N;
+          if (part) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) __stcg(to + c + i, sum[m][i]);
+          } else {
+            constexpr int W = RowPack<G, N>::M;
+            RowPack<G, N> o;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              Acc r = sum[m][i] * scale;
+              if (Add) r += widen(old[Add ? q : 0][m].p[i / W].v[i % W]);
+              o.p[i / W].v[i % W] = narrow<G, Acc>(r);
+            }
+            o.store(dtable + key * A.ldt + c);
+          }
+        }
+        if (part) __threadfence();
+        in_first = false;
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int i = 0; i < N; ++i) sum[m][i] = 0;
+      }
+    }
+  }
+  if (!__syncthreads_or(mine && (came_in || goes_on))) return;
+  // Slot 0 is the run that came in, slot 1 one that begins here and goes on.
+  if (x < 2 && mine) {
+    const bool through = came_in && k[0] == k[Chunk - 1];
+    const bool there = x == 0 ? came_in : goes_on && !through;
+    joined[y][x][0] = -1;
+    if (there) {
+      const uint32_t key = x == 0 ? k[0] : k[Chunk - 1];
+      const int head = x == 0 ? chunk - run_reach<Chunk>(keys, A.count, key, chunk, -1) : chunk;
+      const int tail = x == 0 && !(through && goes_on) ? chunk : chunk + run_reach<Chunk>(keys, A.count, key, chunk, 1);
+      unsigned* ticket = A.tickets + static_cast<int64_t>(head) * gridDim.y + blockIdx.y;
+      __threadfence();
+      if (atomicAdd(ticket, 1u) == static_cast<unsigned>(tail - head)) {
+        *ticket = 0u;
+        __threadfence();
+        joined[y][x][0] = head;
+        joined[y][x][1] = tail;
+      }
+    }
+  }
+  __syncthreads();
+  if (!mine) return;
+#pragma unroll 1
+  for (int slot = 0; slot < 2; ++slot) {
+    const int head = joined[y][slot][0], tail = joined[y][slot][1];
+    if (head < 0) continue;
+    const uint32_t key = slot == 0 ? k[0] : k[Chunk - 1];
+#pragma unroll 1
+    for (int m = 0; m < M; ++m) {
+      const int v = v0 + m * A.across;
+      if (v >= A.packs) continue;
+      const int64_t c = static_cast<int64_t>(v) * N;
+      constexpr int W = RowPack<G, N>::M;
+      RowPack<G, N> o;
+      G* dst = dtable + key * A.ldt + c;
+      if (Add) o.load(dst);
+      Acc sum[N];
+      const Acc* part = parts + (static_cast<int64_t>(head) * 2 + 1) * A.width + c;
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[i] = __ldcg(part + i);
+      part += A.width;  // slot 0 of the next chunk
+#pragma unroll 4
+      for (int q = head + 1; q <= tail; ++q) {
+        const Acc* from = part + static_cast<int64_t>(q - head - 1) * 2 * A.width;
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] += __ldcg(from + i);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        Acc r = sum[i] * scale;
+        if (Add) r += widen(o.p[i / W].v[i % W]);
+        o.p[i / W].v[i % W] = narrow<G, Acc>(r);
+      }
+      o.store(dst);
+    }
+  }
+}
+
+int bits_of(uint64_t v) {
+  int b = 0;
+  while (v >> b) ++b;
+  return b;
 }
 
 }  // namespace
@@ -241,33 +654,68 @@ spmvb_status SortSpace::alloc(int64_t entries) {
   }
   SPMVB_TRY(counts.alloc(static_cast<size_t>(tiles) * kDigits * 4));
   SPMVB_TRY(totals.alloc(kDigits * 4));
-  cap = entries;
   return SPMVB_OK;
 }
 
-spmvb_status sort_entries(SortSpace& space, const int* idx, int64_t count, int n, int* err, cudaStream_t s, Sorted* out) {
+namespace {
+
+// The empty rows shared out among about `blocks` blocks, `most` to one at
+// most; returns the blocks.
+int share_rows(EmptyRows& Z, int blocks, int most) {
+  if (!Z.table) return 0;
+  Z.per_block = static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, ceil_div(Z.rows, blocks))));
+  return static_cast<int>(ceil_div(Z.rows, Z.per_block));
+}
+
+spmvb_status launch_empty_rows(EmptyRows Z, const int* tokens, int count, int sm_count, cudaStream_t s) {
+  const int blocks = share_rows(Z, sm_count * 8, kMaxEmptyRows);
+  write_empty_rows<<<blocks, 256, 0, s>>>(tokens, count, Z);
+  count_launch();
+  SPMVB_TRY_CUDA(cudaGetLastError());
+  return SPMVB_OK;
+}
+
+// Sorts the tokens by row (idx[i] where it is in [0, n), else n, an index past
+// the end reported in *err) and writes the empty rows (if Z.table).
+spmvb_status order_and_clear(SortSpace& space, const int* idx, int count, int n, EmptyRows Z, int sm_count, int* err,
+                             cudaStream_t s, Sorted* out) {
+  const int bits = std::max(1, bits_of(n)), token_bits = bits_of(count - 1);
+  uint32_t* keys0 = space.keys[0].as<uint32_t>();
+  int* vals0 = space.vals[0].as<int>();
+  out->keys = keys0;
+  out->entries = vals0;
+  const bool ranked = count <= kRankTokens && bits + token_bits <= 32;
+  if (count <= kBlockTokens && (Z.table || !ranked)) {
+    const int blocks = 1 + share_rows(Z, sm_count - 1, static_cast<int>(kOrderShared) * 8);
+    order_tokens<<<blocks, kOrderThreads, kOrderShared, s>>>(idx, count, n, bits, keys0, vals0, Z, err);
+    count_launch();
+    SPMVB_TRY_CUDA(cudaGetLastError());
+    return SPMVB_OK;
+  }
+  if (Z.table) SPMVB_TRY(launch_empty_rows(Z, idx, count, sm_count, s));
+  if (ranked) {
+    rank_tokens<<<static_cast<int>(ceil_div(count, 64)), 256, 0, s>>>(idx, count, n, token_bits, keys0, vals0, err);
+    count_launch();
+    SPMVB_TRY_CUDA(cudaGetLastError());
+    return SPMVB_OK;
+  }
   const int tiles = static_cast<int>(ceil_div(count, kTile));
-  int bits = 1;
-  while (bits < 32 && (static_cast<uint64_t>(n) >> bits) != 0) ++bits;
+  const bool scanned = tiles > kOwnTiles;
   int* counts = space.counts.as<int>();
   int* totals = space.totals.as<int>();
   int at = 0;
   for (int shift = 0; shift < bits; shift += kDigitBits, at ^= 1) {
     const bool first = shift == 0;
-    const void* src = first ? static_cast<const void*>(idx) : space.keys[at ^ 1].get();
+    const int* src = first ? idx : space.keys[at ^ 1].as<int>();
     const int* vals = space.vals[at ^ 1].as<int>();
     uint32_t* dk = space.keys[at].as<uint32_t>();
     int* dv = space.vals[at].as<int>();
-    if (first) {
-      digit_counts<true><<<tiles, kSortThreads, 0, s>>>(src, count, n, shift, tiles, counts, err);
-      digit_scan<<<kDigits / 8, 256, 0, s>>>(counts, tiles, totals);
-      digit_scatter<true><<<tiles, kSortThreads, 0, s>>>(src, vals, count, n, shift, tiles, counts, totals, dk, dv, err);
-    } else {
-      digit_counts<false><<<tiles, kSortThreads, 0, s>>>(src, count, n, shift, tiles, counts, err);
-      digit_scan<<<kDigits / 8, 256, 0, s>>>(counts, tiles, totals);
-      digit_scatter<false><<<tiles, kSortThreads, 0, s>>>(src, vals, count, n, shift, tiles, counts, totals, dk, dv, err);
-    }
-    count_launch(3);
+    const auto count_kernel = first ? digit_counts<true> : digit_counts<false>;
+    const auto scatter_kernel = first ? digit_scatter<true> : digit_scatter<false>;
+    count_kernel<<<tiles, kSortThreads, 0, s>>>(src, count, n, shift, tiles, counts, err);
+    if (scanned) digit_scan<<<kDigits / 8, 256, 0, s>>>(counts, tiles, totals);
+    scatter_kernel<<<tiles, kSortThreads, 0, s>>>(src, vals, count, n, shift, tiles, scanned, counts, totals, dk, dv, err);
+    count_launch(scanned ? 3 : 2);
     out->keys = dk;
     out->entries = dv;
   }
@@ -275,34 +723,80 @@ spmvb_status sort_entries(SortSpace& space, const int* idx, int64_t count, int n
   return SPMVB_OK;
 }
 
+}  // namespace
 }  // namespace spmvb
 
 struct spmvb_embedding_st {
   spmvb_context ctx = nullptr;
   int device = 0, rows = 0, width = 0, max_tokens = 0;
   spmvb::SortSpace sort;
-  spmvb::DevBuf parts;  // 2 rows of sums (fp64 wide) per chunk
+  spmvb::DevBuf parts;    // 2 rows of sums (fp64 wide) per chunk
+  spmvb::DevBuf tickets;  // one per chunk and column range
 };
 
 using namespace spmvb;
 
 namespace {
 
-template <typename T, typename G, int VB>
-spmvb_status lookup_grad(spmvb_embedding E, const Sorted& sorted, int count, double scale, const RowSet& dout,
-                         const RowSet& dtable, bool accumulate, cudaStream_t s) {
+template <typename T, typename G, int N>
+spmvb_status lookup_grad(spmvb_embedding E, const Sorted& sorted, EmptyRows Z, const int* tokens, int count, double scale,
+                         const RowSet& dout, const RowSet& dtable, bool accumulate, cudaStream_t s) {
   using Acc = typename AccOf<T>::type;
-  const int packs = E->width / Pack<T, VB>::N;
-  const int chunks = static_cast<int>(ceil_div(count, kChunk));
-  G* dt = static_cast<G*>(const_cast<void*>(dtable.p));
-  run_sums<T, G, VB><<<dim3(chunks, static_cast<unsigned>(ceil_div(packs, kGradThreads))), kGradThreads, 0, s>>>(
-      sorted.keys, sorted.entries, count, E->rows, static_cast<const T*>(dout.p), dout.ld, Acc(scale), dt, dtable.ld,
-      packs, E->width, accumulate, E->parts.as<Acc>());
-  join_runs<T, G><<<dim3(chunks, static_cast<unsigned>(ceil_div(E->width, kGradThreads))), kGradThreads, 0, s>>>(
-      sorted.keys, count, E->rows, Acc(scale), dt, dtable.ld, E->width, accumulate, E->parts.as<Acc>());
-  count_launch(2);
+  constexpr int M = packs_of(N * sizeof(T));
+  const bool self = !sorted.keys;
+  GradView A{};
+  A.keys = sorted.keys;
+  A.vals = sorted.entries;
+  A.tokens = tokens;
+  A.count = count;
+  A.rows = E->rows;
+  A.width = E->width;
+  A.packs = E->width / N;
+  A.across = kMinAcross;
+  while (A.across * M < A.packs && A.across < kGradThreads) A.across *= 2;
+  A.chunks = static_cast<int>(ceil_div(count, chunk_of(self)));
+  A.chunk_blocks = static_cast<int>(ceil_div(A.chunks, kGradThreads / A.across));
+  A.ldo = dout.ld;
+  A.ldt = dtable.ld;
+  A.parts = E->parts.get();
+  A.tickets = E->tickets.as<unsigned>();
+  A.err = E->ctx->index_err();
+  const unsigned ranges = static_cast<unsigned>(ceil_div(A.packs, A.across * M));
+  // Without a sort before it the kernel writes the empty rows too; they are
+  // whole rows, so where it takes the columns in ranges they have a launch.
+  unsigned blocks = A.chunk_blocks;
+  if (self && Z.table && ranges == 1) {
+    blocks += share_rows(Z, E->ctx->sm_count * 8, kSelfTokens * 32);
+    A.empty = Z;
+  } else if (self && Z.table) {
+    SPMVB_TRY(launch_empty_rows(Z, tokens, count, E->ctx->sm_count, s));
+  }
+  if (blocks == 0) return SPMVB_OK;
+  const auto kernel = self ? (accumulate ? grad_rows<T, G, N, true, true> : grad_rows<T, G, N, true, false>)
+                           : (accumulate ? grad_rows<T, G, N, false, true> : grad_rows<T, G, N, false, false>);
+  kernel<<<dim3(blocks, ranges), kGradThreads, 0, s>>>(A, static_cast<const T*>(dout.p), Acc(scale),
+                                                       static_cast<G*>(const_cast<void*>(dtable.p)));
+  count_launch();
   SPMVB_TRY_CUDA(cudaGetLastError());
   return SPMVB_OK;
+}
+
+// Calls lookup_grad for the values of a pack that both row sets allow.
+template <typename T, typename G>
+spmvb_status lookup_grad_by_pack(int n, spmvb_embedding E, const Sorted& sorted, const EmptyRows& Z, const int* tokens,
+                                 int count, double scale, const RowSet& dout, const RowSet& dtable, bool accumulate,
+                                 cudaStream_t s) {
+  switch (n) {
+    case 8:
+      if constexpr (sizeof(T) == 2) return lookup_grad<T, G, 8>(E, sorted, Z, tokens, count, scale, dout, dtable, accumulate, s);
+      break;
+    case 4:
+      if constexpr (sizeof(T) <= 4) return lookup_grad<T, G, 4>(E, sorted, Z, tokens, count, scale, dout, dtable, accumulate, s);
+      break;
+    case 2: return lookup_grad<T, G, 2>(E, sorted, Z, tokens, count, scale, dout, dtable, accumulate, s);
+    case 1: return lookup_grad<T, G, 1>(E, sorted, Z, tokens, count, scale, dout, dtable, accumulate, s);
+  }
+  return fail(SPMVB_ERR_INVALID_ARGUMENT, "row not aligned to its elements");
 }
 
 }  // namespace
@@ -324,7 +818,11 @@ spmvb_status spmvb_embedding_create(spmvb_context ctx, int32_t rows, int32_t wid
     E->width = width;
     E->max_tokens = max_tokens;
     SPMVB_TRY(E->sort.alloc(max_tokens));
-    SPMVB_TRY(E->parts.alloc(static_cast<size_t>(ceil_div(max_tokens, kChunk)) * 2 * width * 8));
+    SPMVB_TRY_CUDA(cudaFuncSetAttribute(order_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize, kOrderShared));
+    const size_t chunks = static_cast<size_t>(
+        std::max(ceil_div(max_tokens, chunk_of(false)), ceil_div(std::min(max_tokens, kSelfTokens), chunk_of(true))));
+    SPMVB_TRY(E->parts.alloc(chunks * 2 * width * 8));
+    SPMVB_TRY(E->tickets.alloc(chunks * ceil_div(width, kGradThreads) * 4));
     *out = E.release();
     return SPMVB_OK;
   });
@@ -375,20 +873,37 @@ spmvb_status spmvb_embedding_lookup_grad(spmvb_embedding E, spmvb_dtype dtype, i
   DeviceGuard g(dev);
   for (const RowSet* r : {&idx, &dout, &dtable}) SPMVB_TRY(check_rows(*r, dev));
   for (const RowSet* r : {&idx, &dout}) SPMVB_TRY(check_apart(dtable, *r));
-  if (!accumulate)
-    SPMVB_TRY_CUDA(cudaMemset2DAsync(d_dtable, ld_dtable * dtable.elem, 0, E->width * dtable.elem, E->rows, s));
-  if (count == 0) return SPMVB_OK;
-  Sorted sorted{};
-  SPMVB_TRY(sort_entries(E->sort, d_tokens, count, E->rows, E->ctx->index_err(), s, &sorted));
-  const int vb = access_bytes(dout.elem, {{dout.p, dout.ld}}, E->width);
-  return with_type<true>(dtype, vb, [&](auto tv, auto vbc) -> spmvb_status {
+  EmptyRows Z{};
+  if (!accumulate) {
+    Z.table = static_cast<char*>(d_dtable);
+    Z.pitch = ld_dtable * static_cast<int64_t>(dtable.elem);
+    Z.bytes = E->width * static_cast<int64_t>(dtable.elem);
+    Z.rows = E->rows;
+    Z.wide = access_bytes(dtable.elem, {{dtable.p, dtable.ld}}, E->width) == 16;
+    Z.elem = dtable.elem == 2 ? 2 : 4;
+  }
+  Sorted sorted{};  // no keys: the kernel sorts
+  if (count > kSelfTokens || (count > 0 && E->rows >= (1 << 23)))
+    SPMVB_TRY(order_and_clear(E->sort, d_tokens, count, E->rows, Z, E->ctx->sm_count, E->ctx->index_err(), s, &sorted));
+  // Values of a pack: dout's rows allow one access for them, dtable's 16-byte
+  // accesses or one.
+  int n = access_bytes(dout.elem, {{dout.p, dout.ld}}, E->width) / static_cast<int>(dout.elem);
+  const int vg = access_bytes(dtable.elem, {{dtable.p, dtable.ld}}, E->width);
+  if (vg < 16) n = std::min(n, vg / static_cast<int>(dtable.elem));
+  const bool add = accumulate != 0;
+  const auto run = [&](auto tv) -> spmvb_status {
     using T = decltype(tv);
-    constexpr int VB = decltype(vbc)::value;
-    if (grad_dtype == dtype) return lookup_grad<T, T, VB>(E, sorted, count, scale, dout, dtable, accumulate != 0, s);
+    if (grad_dtype == dtype) return lookup_grad_by_pack<T, T>(n, E, sorted, Z, d_tokens, count, scale, dout, dtable, add, s);
     if constexpr (sizeof(T) == 2)
-      return lookup_grad<T, float, VB>(E, sorted, count, scale, dout, dtable, accumulate != 0, s);
+      return lookup_grad_by_pack<T, float>(n, E, sorted, Z, d_tokens, count, scale, dout, dtable, add, s);
     return fail(SPMVB_ERR_INVALID_ARGUMENT, "bad dtype");
-  });
+  };
+  switch (dtype) {
+    case SPMVB_F32: return run(float{});
+    case SPMVB_F64: return run(double{});
+    case SPMVB_F16: return run(__half{});
+    default: return run(__nv_bfloat16{});
+  }
 }
 
 }  // extern "C"

@@ -156,22 +156,6 @@ spmvb_status constructed(F&& f) {
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// ---- stable sort of entries by key (segment.cu) ---------------------------------
-// Scratch of sort_entries for up to `cap` entries.
-struct SortSpace {
-  DevBuf keys[2], vals[2], counts, totals;
-  int64_t cap = 0;
-  spmvb_status alloc(int64_t entries);
-};
-struct Sorted {
-  const uint32_t* keys;  // ascending; `n` for entries that select nothing
-  const int* entries;    // in entry order among equal keys
-};
-// Sorts entries 0..count-1 by their key: idx[i] where it is in [0, n), else n
-// (an index >= n is reported in *err). `space` holds the result until its
-// next use.
-spmvb_status sort_entries(SortSpace& space, const int* idx, int64_t count, int n, int* err, cudaStream_t s, Sorted* out);
-
 // ---- row products (rows.cu) ------------------------------------------------------
 // out[t] = scale * sum_j w[t,j] * X[idx[t,j]], j < k (w null: 1).
 spmvb_status launch_lookup(spmvb_dtype dtype, const int* idx, const float* w, int count, int k, int rows, double scale,
