@@ -6,30 +6,30 @@
 //                       token's place is the number of smaller (row, token)
 //                       pairs, 0.5 us of comparisons against a launch of 2.5
 //   up to kRankTokens   the same ranks, by a kernel of one block per 64 tokens
-//   up to kBlockTokens  least-significant-digit radix sort by one block, in
-//                       shared memory
-//   more                the same by many: every tile of kTile tokens counts its
-//                       digits (digit_counts), then ranks its tokens among the
-//                       equal digits before them and writes them to their
-//                       places (digit_scatter), which adds up the tiles'
-//                       counts itself up to kOwnTiles tiles and has them
-//                       summed by digit_scan beyond.
+//   up to kBlockTokens  grouped by a hash of the row (order_tokens), then by
+//                       row: the gradient needs equal rows to be neighbours,
+//                       not the rows in order
+//   more                least-significant-digit radix sort: every tile of
+//                       kTile tokens counts its digits (digit_counts), then
+//                       ranks its tokens among the equal digits before them
+//                       and writes them to their places (digit_scatter),
+//                       which adds up the tiles' counts itself up to kOwnTiles
+//                       tiles and has them summed by digit_scan beyond.
 // Ranks follow the tokens' order, so the order is stable and nothing depends
 // on timing.
 //
 // Gradient. dtable[r] = scale * sum of dout[t] over the tokens that name r:
-// in sorted order the tokens of one row are neighbours (a run). A block takes
-// chunks of kChunk sorted tokens and a range of columns, adds each run in
-// registers and writes the runs that lie inside a chunk. A run that crosses a
-// chunk's edge leaves its part in scratch (slot 0: the run came in from the
-// chunk before, slot 1: it begins here and goes on); the last of its blocks to
-// arrive adds the parts in chunk order. A frequent token is so spread over
+// in that order the tokens of one row are neighbours (a run). A block takes
+// chunks of 16 or 4 tokens and a range of columns and adds each run in
+// registers. A run no longer than a chunk belongs to the chunk where it begins,
+// whole. Of a longer one every chunk that holds some leaves its part in scratch (slot 0: the run came
+// in from the chunk before, slot 1: it begins here and goes on); the last of
+// its blocks to arrive adds the parts in chunk order. A frequent token is so spread over
 // many blocks, in a fixed order of summation. Where the gradient is not added
 // to what is there, the rows that no token names are written as well
-// (empty_rows), in the launch that sorts: its other blocks find the rows named
-// in their range by reading all tokens, so the sort takes no time of its own.
-// The table is written once, and that bounds the kernels (1.07 GB of 1.2 GB
-// for 16,384 tokens of 4,096 bf16 values and 131,072 rows).
+// (empty_rows), by blocks of their own after those of the sums; which rows are
+// named, the sort notes in a bit each. The table is written once, and that bounds the kernels
+// (1.07 GB of 1.2 GB for 16,384 tokens of 4,096 bf16 values and 131,072 rows).
 #include "select.cuh"
 
 namespace spmvb {
@@ -54,6 +54,7 @@ constexpr int kPerThread = 4;
 constexpr int kTile = kSortThreads * kPerThread;
 constexpr int kOwnTiles = 64;
 constexpr int kSelfTokens = 256;
+constexpr int kGradThreads = 256;
 constexpr int kRankTokens = 2048;
 constexpr int kBlockTokens = 16384;
 constexpr int kOrderThreads = 1024;
@@ -65,11 +66,64 @@ __device__ __forceinline__ uint32_t key_of(int i, uint32_t n, int* err) {
   return i < 0 || static_cast<uint32_t>(i) >= n ? n : static_cast<uint32_t>(i);
 }
 
+// Rows that no token names, a few to a block: pieces of 8 to 64 KB written in
+// their order reach 7.4 TB/s, 1 MB a block 6.1.
+constexpr int kEmptyRows = 8, kMaxEmptyRows = 256;
+struct EmptyRows {
+  char* table;           // null: nothing to write
+  int64_t pitch, bytes;  // of a row
+  int rows, per_block;   // rows of a block: a multiple of kEmptyRows
+  bool wide;             // 16 bytes at a time, else `elem`
+  int elem;
+  uint8_t* named;        // a bit per row, set by the sort; null: look the tokens through
+};
+
+__device__ __forceinline__ void name_row(uint32_t* named, uint32_t row, uint32_t rows) {
+  if (named && row < rows) atomicOr(named + (row >> 5), 1u << (row & 31));
+}
+
+// A block's rows, a warp a row. The bits are cleared for the next call.
+__device__ __forceinline__ void empty_rows(const EmptyRows& Z, int block, const int* __restrict__ tokens, int count) {
+  __shared__ unsigned bits[kMaxEmptyRows / kEmptyRows];  // 8 rows each
+  const int64_t r0 = static_cast<int64_t>(block) * Z.per_block;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, bytes = Z.per_block / kEmptyRows;
+  if (static_cast<int>(threadIdx.x) < bytes) {
+    const int64_t at = r0 / kEmptyRows + threadIdx.x;
+    const bool in = Z.named && at * kEmptyRows < Z.rows;
+    bits[threadIdx.x] = in ? Z.named[at] : 0u;
+    if (in && bits[threadIdx.x]) Z.named[at] = 0;
+  }
+  __syncthreads();
+  if (!Z.named) {
+    for (int i = threadIdx.x; i < count; i += kGradThreads) {
+      const int64_t r = __ldg(tokens + i) - r0;
+      if (r >= 0 && r < Z.per_block) atomicOr(&bits[r / kEmptyRows], 1u << (r % kEmptyRows));
+    }
+    __syncthreads();
+  }
+  for (int q = 0; q < bytes; ++q) {
+    const int64_t r = r0 + q * kEmptyRows + w;
+    if (r >= Z.rows || (bits[q] >> w & 1u)) continue;
+    char* row = Z.table + r * Z.pitch;
+    if (Z.wide) {
+#pragma unroll 4
+      for (int64_t i = lane; i < Z.bytes / 16; i += 32) __stcs(reinterpret_cast<uint4*>(row) + i, make_uint4(0, 0, 0, 0));
+    } else if (Z.elem == 2) {
+#pragma unroll 4
+      for (int64_t i = lane; i < Z.bytes / 2; i += 32) __stcs(reinterpret_cast<uint16_t*>(row) + i, uint16_t(0));
+    } else {
+#pragma unroll 4
+      for (int64_t i = lane; i < Z.bytes / 4; i += 32) __stcs(reinterpret_cast<uint32_t*>(row) + i, 0u);
+    }
+  }
+}
+static_assert(kEmptyRows == kGradThreads / 32 && kEmptyRows == 8);
+
 // counts[digit * tiles + tile].
 template <bool First>
 __global__ void __launch_bounds__(kSortThreads)
     digit_counts(const int* __restrict__ src, int64_t count, uint32_t n, int shift, int tiles, int* __restrict__ counts,
-                 int* __restrict__ err) {
+                 uint32_t* __restrict__ named, int* __restrict__ err) {
   __shared__ int c[kDigits];
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) c[d] = 0;
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kTile + threadIdx.x;
@@ -80,7 +134,10 @@ __global__ void __launch_bounds__(kSortThreads)
 #pragma unroll
   for (int q = 0; q < kPerThread; ++q) {
     const uint32_t key = First ? key_of(raw[q], n, err) : static_cast<uint32_t>(raw[q]);
-    if (i0 + q * kSortThreads < count) atomicAdd(&c[(key >> shift) & (kDigits - 1)], 1);
+    if (i0 + q * kSortThreads < count) {
+      atomicAdd(&c[(key >> shift) & (kDigits - 1)], 1);
+      if (First) name_row(named, key, n);
+    }
   }
   __syncthreads();
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) counts[static_cast<int64_t>(d) * tiles + blockIdx.x] = c[d];
@@ -236,7 +293,7 @@ __device__ __forceinline__ int rank_among(uint32_t mine, const uint32_t* pairs, 
 // Sorted keys and tokens by counting: 64 tokens a block, 4 threads a token.
 __global__ void __launch_bounds__(256)
     rank_tokens(const int* __restrict__ src, int count, uint32_t n, int token_bits, uint32_t* __restrict__ keys,
-                int* __restrict__ vals, int* __restrict__ err) {
+                int* __restrict__ vals, uint32_t* __restrict__ named, int* __restrict__ err) {
   __shared__ __align__(16) uint32_t pairs[kRankTokens];
   const int padded = (count + 3) / 4 * 4;
 #pragma unroll 4
@@ -251,12 +308,11 @@ __global__ void __launch_bounds__(256)
   if (i < count && (threadIdx.x & 3) == 0) {
     keys[at] = pairs[i] >> token_bits;
     vals[at] = i;
-    key_of(__ldg(src + i), n, err);  // reports an index past the end
+    name_row(named, key_of(__ldg(src + i), n, err), n);
   }
 }
 
 // ---- embedding gradient ----------------------------------------------------------
-constexpr int kGradThreads = 256;
 constexpr int kMinAcross = 8;  // threads along a row, at least
 
 // N values of a row, by accesses of up to 16 bytes; the row is aligned to them.
@@ -275,91 +331,119 @@ struct RowPack {
   }
 };
 
-struct EmptyRows {
-  char* table;           // null: nothing to write
-  int64_t pitch, bytes;  // of a row
-  int rows, per_block;   // rows of a block
-  bool wide;             // 16 bytes at a time, else `elem`
-  int elem;
-};
-
-// The rows of one block's range that no token names, a warp a row. `named`: a
-// bit per row of the range.
-__device__ __forceinline__ void empty_rows(const EmptyRows& Z, int block, const int* __restrict__ tokens, int count,
-                                           uint32_t* named) {
-  const int r0 = block * Z.per_block, r1 = min(r0 + Z.per_block, Z.rows), lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < (Z.per_block + 31) / 32; i += blockDim.x) named[i] = 0u;
-  __syncthreads();
-#pragma unroll 4
-  for (int i = threadIdx.x; i < count; i += blockDim.x) {
-    const int r = __ldg(tokens + i);
-    if (r >= r0 && r < r1) atomicOr(&named[(r - r0) >> 5], 1u << ((r - r0) & 31));
-  }
-  __syncthreads();
-  const int warps = blockDim.x >> 5;
-  for (int r = r0 + (threadIdx.x >> 5); r < r1; r += warps) {
-    if (named[(r - r0) >> 5] >> ((r - r0) & 31) & 1u) continue;
-    char* row = Z.table + r * Z.pitch;
-    if (Z.wide) {
-#pragma unroll 4
-      for (int64_t i = lane; i < Z.bytes / 16; i += 32) __stcs(reinterpret_cast<uint4*>(row) + i, make_uint4(0, 0, 0, 0));
-    } else if (Z.elem == 2) {
-#pragma unroll 4
-      for (int64_t i = lane; i < Z.bytes / 2; i += 32) __stcs(reinterpret_cast<uint16_t*>(row) + i, uint16_t(0));
-    } else {
-#pragma unroll 4
-      for (int64_t i = lane; i < Z.bytes / 4; i += 32) __stcs(reinterpret_cast<uint32_t*>(row) + i, 0u);
-    }
-  }
-}
-constexpr int kMaxEmptyRows = 8192;  // of a block: 1 KB of bits
-
-// Block 0 sorts up to kBlockTokens tokens; the others write the empty rows.
+// Groups up to kBlockTokens tokens by row: block p < parts (a power of two)
+// takes the rows whose hash is p, in the order of the tokens, and sorts them by
+// row; its place in the result is the number of tokens of smaller hash. The
+// hash spreads the frequent tokens, which have neighbouring numbers.
 // Shared memory: keys, 16-bit tokens, 16-bit counts per warp and digit.
 constexpr size_t kOrderShared = kBlockTokens * 6 + (kOrderThreads / 32) * kDigits * 2;
+constexpr int kRankGroup = 512;  // tokens of a block ranked by counting; more by digits
 __global__ void __launch_bounds__(kOrderThreads)
-    order_tokens(const int* __restrict__ src, int count, uint32_t n, int bits, uint32_t* __restrict__ keys,
-                 int* __restrict__ vals, EmptyRows Z, int* __restrict__ err) {
+    order_tokens(const int* __restrict__ src, int count, uint32_t n, int bits, int parts, int hash_shift,
+                 uint32_t* __restrict__ keys, int* __restrict__ vals, uint32_t* __restrict__ named, int* __restrict__ err) {
   extern __shared__ __align__(16) uint32_t shared[];
-  if (blockIdx.x > 0) {
-    empty_rows(Z, blockIdx.x - 1, src, count, shared);
-    return;
-  }
+  const int part = blockIdx.x;
   constexpr int Warps = kOrderThreads / 32, Rounds = kBlockTokens / kOrderThreads;
   uint32_t* sk = shared;
   uint16_t* sv = reinterpret_cast<uint16_t*>(shared + kBlockTokens);
   uint16_t* wc = sv + kBlockTokens;
-  __shared__ int sh[kDigits / 32];
+  __shared__ int sh[kDigits / 32], found[3][Warps];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int rounds = (count + kOrderThreads - 1) / kOrderThreads;  // of 32 tokens a warp, neighbours
-  const int i0 = w * rounds * 32 + lane;
+  const unsigned before_me = (1u << lane) - 1u;
   uint32_t key[Rounds], place[Rounds];  // place: token << 16 | rank
+  int m;  // tokens of this block
+  {
+    const int turns = (count + kOrderThreads - 1) / kOrderThreads;  // of 32 tokens a warp, neighbours
+    const int i0 = w * turns * 32 + lane;
 #pragma unroll
-  for (int q = 0; q < Rounds; ++q)
-    key[q] = q < rounds && i0 + q * 32 < count ? static_cast<uint32_t>(__ldg(src + i0 + q * 32)) : 0u;
+    for (int q = 0; q < Rounds; ++q)
+      key[q] = q < turns && i0 + q * 32 < count ? static_cast<uint32_t>(__ldg(src + i0 + q * 32)) : 0xffffffffu;
+    int own = 0, less = 0, all = 0;
 #pragma unroll
-  for (int q = 0; q < Rounds; ++q) {
-    key[q] = key_of(static_cast<int>(key[q]), n, err);
-    place[q] = static_cast<uint32_t>(i0 + q * 32) << 16;
+    for (int q = 0; q < Rounds; ++q) {
+      if (q >= turns) break;
+      if (part == 0) key_of(static_cast<int>(key[q]), n, err);  // reports an index past the end
+      const bool in = key[q] < n;
+      const int hash = static_cast<int>(key[q] * 2654435761u >> hash_shift);
+      own += __popc(__ballot_sync(0xffffffffu, in && hash == part));
+      less += __popc(__ballot_sync(0xffffffffu, in && hash < part));
+      all += __popc(__ballot_sync(0xffffffffu, in));
+    }
+    if (lane == 0) {
+      found[0][w] = own;
+      found[1][w] = less;
+      found[2][w] = all;
+    }
+    __syncthreads();
+    int incl = found[0][lane], offset = found[1][lane];
+    const int here = incl;
+    all = found[2][lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += u;
+      offset += __shfl_xor_sync(0xffffffffu, offset, off);
+      all += __shfl_xor_sync(0xffffffffu, all, off);
+    }
+    m = __shfl_sync(0xffffffffu, incl, 31);
+    int at = __shfl_sync(0xffffffffu, incl - here, w);
+#pragma unroll
+    for (int q = 0; q < Rounds; ++q) {
+      if (q >= turns) break;
+      const bool in = key[q] < n && static_cast<int>(key[q] * 2654435761u >> hash_shift) == part;
+      const unsigned vote = __ballot_sync(0xffffffffu, in);
+      if (in) {
+        name_row(named, key[q], n);
+        sk[at + __popc(vote & before_me)] = key[q];
+        sv[at + __popc(vote & before_me)] = static_cast<uint16_t>(i0 + q * 32);
+      }
+      at += __popc(vote);
+    }
+    keys += offset;
+    vals += offset;
+    // The tokens that select nothing come after all others.
+    if (part == parts - 1)
+      for (int i = all + threadIdx.x; i < count; i += kOrderThreads) {
+        keys[i - offset] = n;
+        vals[i - offset] = 0;
+      }
+    __syncthreads();
   }
+  if (m <= kRankGroup && bits <= 23) {
+    uint32_t* pairs = reinterpret_cast<uint32_t*>(wc);  // row << 9 | place in the list
+    const int padded = (m + 3) / 4 * 4;
+    if (static_cast<int>(threadIdx.x) < padded)
+      pairs[threadIdx.x] = static_cast<int>(threadIdx.x) < m ? sk[threadIdx.x] << 9 | threadIdx.x : 0xffffffffu;
+    __syncthreads();
+    if (m == 0) return;
+    int each = 2;  // threads of a token
+    while (each < 32 && m * each * 2 <= kOrderThreads) each *= 2;
+    const int i = threadIdx.x / each;
+    const int at = rank_among(pairs[min(i, m - 1)], pairs, m, each, threadIdx.x % each);
+    if (i < m && threadIdx.x % each == 0) {
+      keys[at] = sk[i];
+      vals[at] = sv[i];
+    }
+    return;
+  }
+  const int rounds = (m + kOrderThreads - 1) / kOrderThreads;
+  const int i0 = w * rounds * 32 + lane;
   for (int shift = 0; shift < bits; shift += kDigitBits) {
     uint32_t* zero = reinterpret_cast<uint32_t*>(wc);
     for (int i = threadIdx.x; i < Warps * kDigits / 2; i += kOrderThreads) zero[i] = 0u;
     __syncthreads();
-    if (shift > 0) {
 #pragma unroll
-      for (int q = 0; q < Rounds; ++q)
-        if (q < rounds && i0 + q * 32 < count) {
-          key[q] = sk[i0 + q * 32];
-          place[q] = static_cast<uint32_t>(sv[i0 + q * 32]) << 16;
-        }
+    for (int q = 0; q < Rounds; ++q) {
+      const bool in = q < rounds && i0 + q * 32 < m;
+      key[q] = in ? sk[i0 + q * 32] : 0u;
+      place[q] = in ? static_cast<uint32_t>(sv[i0 + q * 32]) << 16 : 0u;
     }
     uint16_t* mine = wc + w * kDigits;
 #pragma unroll
     for (int q = 0; q < Rounds; ++q) {
       if (q >= rounds) break;
       // The lanes with the same digit, from one vote a bit.
-      const bool in = i0 + q * 32 < count;
+      const bool in = i0 + q * 32 < m;
       unsigned same = __ballot_sync(0xffffffffu, in);
 #pragma unroll
       for (int bit = 0; bit < kDigitBits; ++bit) {
@@ -368,7 +452,7 @@ __global__ void __launch_bounds__(kOrderThreads)
         same &= on ? vote : ~vote;
       }
       const int d = static_cast<int>((key[q] >> shift) & (kDigits - 1));
-      const unsigned before = same & ((1u << lane) - 1u);
+      const unsigned before = same & before_me;
       const int base = mine[d];
       __syncwarp();
       if (in && before == 0) mine[d] = static_cast<uint16_t>(base + __popc(same));
@@ -405,7 +489,7 @@ __global__ void __launch_bounds__(kOrderThreads)
     const bool last = shift + kDigitBits >= bits;
 #pragma unroll
     for (int q = 0; q < Rounds; ++q) {
-      if (q >= rounds || i0 + q * 32 >= count) continue;
+      if (q >= rounds || i0 + q * 32 >= m) continue;
       const int at = mine[(key[q] >> shift) & (kDigits - 1)] + static_cast<int>(place[q] & 0xffffu);
       if (last) {
         keys[at] = key[q];
@@ -419,23 +503,19 @@ __global__ void __launch_bounds__(kOrderThreads)
   }
 }
 
-__global__ void __launch_bounds__(256) write_empty_rows(const int* __restrict__ src, int count, EmptyRows Z) {
-  __shared__ uint32_t named[kMaxEmptyRows / 32];
-  empty_rows(Z, blockIdx.x, src, count, named);
-}
-
 struct GradView {
   const uint32_t* keys;  // sorted (unless the block sorts)
   const int* vals;
   const int* tokens;
   int count;
   uint32_t rows;
-  int chunks, chunk_blocks;  // blocks of the grid's x that take chunks; the others write empty rows
-  int width, packs, across;  // columns, packs of them, threads along a row
+  int chunks, chunk_blocks;   // blocks of chunks, times `ranges` of columns
+  int ranges, empty_blocks;   // the grid's other blocks write empty rows
+  int width, packs, across;   // columns, packs of them, threads along a row
   int64_t ldo, ldt;
   void* parts;
-  unsigned* tickets;  // chunks x gridDim.y, all 0 between calls
-  EmptyRows empty;    // where the block sorts
+  unsigned* tickets;  // chunks x ranges, all 0 between calls
+  EmptyRows empty;
   int* err;
 };
 
@@ -458,28 +538,37 @@ __device__ __forceinline__ int run_reach(const uint32_t* keys, int count, uint32
   return have;
 }
 
-// Tokens of a chunk: few where there are few, to spread them.
-constexpr int chunk_of(bool self) { return self ? 4 : 16; }
+// Tokens of a chunk: few where they would not fill the GPU.
+constexpr int kChunk = 16, kSmallChunk = 4;
 // Packs of a thread, `across` packs apart: 16 bytes in all, 4 packs at most.
 constexpr int packs_of(int bytes) { return bytes >= 16 ? 1 : 16 / bytes > 4 ? 4 : 16 / bytes; }
 
-template <typename T, typename G, int N, bool Self, bool Add>
-__global__ void __launch_bounds__(kGradThreads)
+template <typename T, typename G, int N, int Chunk, bool Self, bool Add>
+__global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * sizeof(G) > 16) ? 2 : N * sizeof(T) < 16 ? 3 : 4)
     grad_rows(GradView A, const T* __restrict__ dout, typename AccOf<T>::type scale, G* __restrict__ dtable) {
   using Acc = typename AccOf<T>::type;
   constexpr int VB = N * sizeof(T), M = packs_of(VB);
-  constexpr int Chunk = chunk_of(Self);
-  constexpr int Batch = Self || Add ? 4 : 8;  // rows loaded before the first is added
+  constexpr int Batch = 4;  // rows loaded before the first is added
+  constexpr int Span = 3 * Chunk;
+  constexpr int MaxDown = kGradThreads / kMinAcross;
   __shared__ __align__(16) uint32_t pairs[Self ? kSelfTokens : 4];
   __shared__ uint32_t self_keys[Self ? kSelfTokens : 1];
   __shared__ int self_vals[Self ? kSelfTokens : 1];
+  __shared__ uint32_t ck[MaxDown * Span];
+  __shared__ int cv[MaxDown * Span];
+  __shared__ int joined[MaxDown][2][2];  // by slot: first and last chunk of a run whose parts are all there
   const uint32_t* keys = A.keys;
   const int* vals = A.vals;
+  // The blocks that write empty rows come last: their writes run at full rate
+  // in order, and slow down the loads of the others (238 us against 207 where
+  // they were spread among them).
+  const int block = static_cast<int>(blockIdx.x), sums = static_cast<int>(gridDim.x) - A.empty_blocks;
+  if (block >= sums) {
+    empty_rows(A.empty, block - sums, A.tokens, A.count);
+    return;
+  }
+  const int range = block % A.ranges, block_x = block / A.ranges;
   if constexpr (Self) {
-    if (static_cast<int>(blockIdx.x) >= A.chunk_blocks) {
-      empty_rows(A.empty, blockIdx.x - A.chunk_blocks, A.tokens, A.count, self_keys);
-      return;
-    }
     // Rows have at most 23 bits, tokens 8.
     const int padded = (A.count + 3) / 4 * 4;
     for (int i = threadIdx.x; i < padded; i += kGradThreads)
@@ -498,77 +587,100 @@ __global__ void __launch_bounds__(kGradThreads)
     vals = self_vals;
   }
 
-  // A chunk's keys with the one before and the one after it, and its tokens.
-  constexpr int Span = Chunk + 2;
-  constexpr int MaxDown = kGradThreads / kMinAcross;
-  __shared__ uint32_t ck[MaxDown * Span];
-  __shared__ int cv[MaxDown * Span];
-  __shared__ int joined[MaxDown][2][2];  // by slot: first and last chunk of a run whose parts are all there
+  // A chunk's keys and tokens, with the chunk before and the one after it.
   const int down = kGradThreads / A.across;
   const int x = threadIdx.x % A.across, y = threadIdx.x / A.across;
   for (int i = threadIdx.x; i < down * Span; i += kGradThreads) {
-    const int64_t at = (static_cast<int64_t>(blockIdx.x) * down + i / Span) * Chunk + i % Span - 1;
+    const int64_t at = (static_cast<int64_t>(block_x) * down + i / Span - 1) * Chunk + i % Span;
     const bool in = at >= 0 && at < A.count;
     ck[i] = in ? keys[at] : 0xffffffffu;
     cv[i] = in ? vals[at] : 0;
   }
   __syncthreads();
-  const int chunk = blockIdx.x * down + y, v0 = blockIdx.y * A.across * M + x;
-  const uint32_t* k = ck + y * Span + 1;
-  const int* t = cv + y * Span + 1;
+  const int chunk = block_x * down + y, v0 = range * A.across * M + x;
+  const uint32_t* k = ck + y * Span + Chunk;
+  const int* t = cv + y * Span + Chunk;
   Acc* parts = static_cast<Acc*>(A.parts);
   const bool mine = chunk < A.chunks;
-  // Entries that select nothing (key = rows) come last; past the end it is ~0.
-  const bool came_in = k[0] < A.rows && k[-1] == k[0];
-  const bool goes_on = k[Chunk - 1] < A.rows && k[Chunk] == k[Chunk - 1];
+  // The runs that cross the chunk's edges: [first_begin, first_end) and
+  // [last_begin, last_end), as far as they are in view. Tokens that select
+  // nothing (key = rows) and places past the end (~0) are no runs.
+  bool came_in = k[0] < A.rows && k[-1] == k[0];
+  bool goes_on = k[Chunk - 1] < A.rows && k[Chunk] == k[Chunk - 1];
+  int begin = 0, end = Chunk;
+  if (came_in) {
+    int from = -1, to = 1;
+    while (from > -Chunk && k[from - 1] == k[0]) --from;
+    while (to < 2 * Chunk && k[to] == k[0]) ++to;
+    if (to - from <= Chunk) {  // short: the chunk before adds it
+      came_in = false;
+      begin = to;
+    }
+  }
+  const bool through = came_in && k[0] == k[Chunk - 1];
+  if (goes_on) {
+    int from = Chunk - 1, to = Chunk + 1;
+    while (from > -Chunk && k[from - 1] == k[Chunk - 1]) --from;
+    while (to < 2 * Chunk && k[to] == k[Chunk - 1]) ++to;
+    if (to - from <= Chunk) {
+      goes_on = false;
+      end = from < 0 ? Chunk : to;
+    }
+  }
   bool in_first = came_in;
-  const auto ends = [&](int i) { return i == Chunk - 1 || k[i + 1] != k[i]; };
+  int col[M];  // -1: past the row's end
+#pragma unroll
+  for (int m = 0; m < M; ++m) col[m] = v0 + m * A.across < A.packs ? (v0 + m * A.across) * N : -1;
   if (mine) {
     Acc sum[M][N] = {};
-#pragma unroll
-    for (int b = 0; b < Chunk; b += Batch) {
+#pragma unroll 1
+    for (int b = begin; b < end; b += Batch) {
       Pack<T, VB> p[Batch][M];
       RowPack<G, N> old[Add ? Batch : 1][M];
 #pragma unroll
       for (int q = 0; q < Batch; ++q) {
-        if (k[b + q] >= A.rows) continue;
+        const int i = b + q;
+        if (i >= end || k[i] >= A.rows) continue;
+        const T* from = dout + t[i] * A.ldo;
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-          const int v = v0 + m * A.across;
-          if (v >= A.packs) continue;
-          p[q][m] = ld_pack_stream<T, VB>(dout + t[b + q] * A.ldo + static_cast<int64_t>(v) * N);
-          if (Add && ends(b + q)) old[Add ? q : 0][m].load(dtable + k[b + q] * A.ldt + static_cast<int64_t>(v) * N);
+        for (int m = 0; m < M; ++m)
+          if (col[m] >= 0) p[q][m] = ld_pack_stream<T, VB>(from + col[m]);
+        if (Add && (i + 1 == end || k[i + 1] != k[i])) {
+          const G* was = dtable + k[i] * A.ldt;
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+            if (col[m] >= 0) old[Add ? q : 0][m].load(was + col[m]);
         }
       }
 #pragma unroll
       for (int q = 0; q < Batch; ++q) {
-        const uint32_t key = k[b + q];
-        if (key >= A.rows) continue;
+        const int i = b + q;
+        if (i >= end || k[i] >= A.rows) continue;
+        const uint32_t key = k[i];
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int i = 0; i < N; ++i) sum[m][i] += widen(p[q][m].v[i]);
-        if (!ends(b + q)) continue;
-        const bool part = in_first || (b + q == Chunk - 1 && goes_on);
+          for (int n = 0; n < N; ++n) sum[m][n] += widen(p[q][m].v[n]);
+        if (i + 1 < end && k[i + 1] == key) continue;
+        const bool part = in_first || (i == Chunk - 1 && goes_on);
         Acc* to = parts + (static_cast<int64_t>(chunk) * 2 + (in_first ? 0 : 1)) * A.width;
+        G* row = dtable + key * A.ldt;
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-          const int v = v0 + m * A.across;
-          if (v >= A.packs) continue;
-          const int64_t c = static_cast<int64_t>(v) * N;
+          if (col[m] < 0) continue;
           if (part) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) __stcg(to + c + i, sum[m][i]);
+            for (int n = 0; n < N; ++n) __stcg(to + col[m] + n, sum[m][n]);
           } else {
             constexpr int W = RowPack<G, N>::M;
             RowPack<G, N> o;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-              Acc r = sum[m][i] * scale;
-              if (Add) r += widen(old[Add ? q : 0][m].p[i / W].v[i % W]);
-              o.p[i / W].v[i % W] = narrow<G, Acc>(r);
+            for (int n = 0; n < N; ++n) {
+              Acc r = sum[m][n] * scale;
+              if (Add) r += widen(old[Add ? q : 0][m].p[n / W].v[n % W]);
+              o.p[n / W].v[n % W] = narrow<G, Acc>(r);
             }
-            o.store(dtable + key * A.ldt + c);
+            o.store(row + col[m]);
           }
         }
         if (part) __threadfence();
@@ -576,21 +688,20 @@ __global__ void __launch_bounds__(kGradThreads)
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int i = 0; i < N; ++i) sum[m][i] = 0;
+          for (int n = 0; n < N; ++n) sum[m][n] = 0;
       }
     }
   }
   if (!__syncthreads_or(mine && (came_in || goes_on))) return;
   // Slot 0 is the run that came in, slot 1 one that begins here and goes on.
   if (x < 2 && mine) {
-    const bool through = came_in && k[0] == k[Chunk - 1];
     const bool there = x == 0 ? came_in : goes_on && !through;
     joined[y][x][0] = -1;
     if (there) {
       const uint32_t key = x == 0 ? k[0] : k[Chunk - 1];
       const int head = x == 0 ? chunk - run_reach<Chunk>(keys, A.count, key, chunk, -1) : chunk;
       const int tail = x == 0 && !(through && goes_on) ? chunk : chunk + run_reach<Chunk>(keys, A.count, key, chunk, 1);
-      unsigned* ticket = A.tickets + static_cast<int64_t>(head) * gridDim.y + blockIdx.y;
+      unsigned* ticket = A.tickets + static_cast<int64_t>(head) * A.ranges + range;
       __threadfence();
       if (atomicAdd(ticket, 1u) == static_cast<unsigned>(tail - head)) {
         *ticket = 0u;
@@ -609,9 +720,8 @@ __global__ void __launch_bounds__(kGradThreads)
     const uint32_t key = slot == 0 ? k[0] : k[Chunk - 1];
 #pragma unroll 1
     for (int m = 0; m < M; ++m) {
-      const int v = v0 + m * A.across;
-      if (v >= A.packs) continue;
-      const int64_t c = static_cast<int64_t>(v) * N;
+      const int64_t c = static_cast<int64_t>(v0 + m * A.across) * N;
+      if (c >= A.width) continue;
       constexpr int W = RowPack<G, N>::M;
       RowPack<G, N> o;
       G* dst = dtable + key * A.ldt + c;
@@ -659,42 +769,28 @@ spmvb_status SortSpace::alloc(int64_t entries) {
 
 namespace {
 
-// The empty rows shared out among about `blocks` blocks, `most` to one at
-// most; returns the blocks.
-int share_rows(EmptyRows& Z, int blocks, int most) {
-  if (!Z.table) return 0;
-  Z.per_block = static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, ceil_div(Z.rows, blocks))));
-  return static_cast<int>(ceil_div(Z.rows, Z.per_block));
-}
-
-spmvb_status launch_empty_rows(EmptyRows Z, const int* tokens, int count, int sm_count, cudaStream_t s) {
-  const int blocks = share_rows(Z, sm_count * 8, kMaxEmptyRows);
-  write_empty_rows<<<blocks, 256, 0, s>>>(tokens, count, Z);
-  count_launch();
-  SPMVB_TRY_CUDA(cudaGetLastError());
-  return SPMVB_OK;
-}
-
-// Sorts the tokens by row (idx[i] where it is in [0, n), else n, an index past
-// the end reported in *err) and writes the empty rows (if Z.table).
-spmvb_status order_and_clear(SortSpace& space, const int* idx, int count, int n, EmptyRows Z, int sm_count, int* err,
-                             cudaStream_t s, Sorted* out) {
+// Sorts the tokens by row: idx[i] where it is in [0, n), else n (an index past
+// the end is reported in *err). `named` (or null) receives the rows' bits.
+spmvb_status order_tokens_by_row(SortSpace& space, const int* idx, int count, int n, uint32_t* named, int* err,
+                                 cudaStream_t s, Sorted* out) {
   const int bits = std::max(1, bits_of(n)), token_bits = bits_of(count - 1);
   uint32_t* keys0 = space.keys[0].as<uint32_t>();
   int* vals0 = space.vals[0].as<int>();
   out->keys = keys0;
   out->entries = vals0;
   const bool ranked = count <= kRankTokens && bits + token_bits <= 32;
-  if (count <= kBlockTokens && (Z.table || !ranked)) {
-    const int blocks = 1 + share_rows(Z, sm_count - 1, static_cast<int>(kOrderShared) * 8);
-    order_tokens<<<blocks, kOrderThreads, kOrderShared, s>>>(idx, count, n, bits, keys0, vals0, Z, err);
+  if (count <= kBlockTokens && !ranked) {
+    // About 128 tokens a block.
+    int parts_log = 1;
+    while (parts_log < 7 && (128 << parts_log) < count) ++parts_log;
+    order_tokens<<<1 << parts_log, kOrderThreads, kOrderShared, s>>>(idx, count, n, bits, 1 << parts_log, 32 - parts_log,
+                                                                    keys0, vals0, named, err);
     count_launch();
     SPMVB_TRY_CUDA(cudaGetLastError());
     return SPMVB_OK;
   }
-  if (Z.table) SPMVB_TRY(launch_empty_rows(Z, idx, count, sm_count, s));
   if (ranked) {
-    rank_tokens<<<static_cast<int>(ceil_div(count, 64)), 256, 0, s>>>(idx, count, n, token_bits, keys0, vals0, err);
+    rank_tokens<<<static_cast<int>(ceil_div(count, 64)), 256, 0, s>>>(idx, count, n, token_bits, keys0, vals0, named, err);
     count_launch();
     SPMVB_TRY_CUDA(cudaGetLastError());
     return SPMVB_OK;
@@ -712,7 +808,7 @@ spmvb_status order_and_clear(SortSpace& space, const int* idx, int count, int n,
     int* dv = space.vals[at].as<int>();
     const auto count_kernel = first ? digit_counts<true> : digit_counts<false>;
     const auto scatter_kernel = first ? digit_scatter<true> : digit_scatter<false>;
-    count_kernel<<<tiles, kSortThreads, 0, s>>>(src, count, n, shift, tiles, counts, err);
+    count_kernel<<<tiles, kSortThreads, 0, s>>>(src, count, n, shift, tiles, counts, named, err);
     if (scanned) digit_scan<<<kDigits / 8, 256, 0, s>>>(counts, tiles, totals);
     scatter_kernel<<<tiles, kSortThreads, 0, s>>>(src, vals, count, n, shift, tiles, scanned, counts, totals, dk, dv, err);
     count_launch(scanned ? 3 : 2);
@@ -731,7 +827,8 @@ struct spmvb_embedding_st {
   int device = 0, rows = 0, width = 0, max_tokens = 0;
   spmvb::SortSpace sort;
   spmvb::DevBuf parts;    // 2 rows of sums (fp64 wide) per chunk
-  spmvb::DevBuf tickets;  // one per chunk and column range
+  spmvb::DevBuf tickets;  // one per chunk and column range, 0 between calls
+  spmvb::DevBuf named;    // a bit per row, 0 between calls
 };
 
 using namespace spmvb;
@@ -754,28 +851,27 @@ spmvb_status lookup_grad(spmvb_embedding E, const Sorted& sorted, EmptyRows Z, c
   A.packs = E->width / N;
   A.across = kMinAcross;
   while (A.across * M < A.packs && A.across < kGradThreads) A.across *= 2;
-  A.chunks = static_cast<int>(ceil_div(count, chunk_of(self)));
-  A.chunk_blocks = static_cast<int>(ceil_div(A.chunks, kGradThreads / A.across));
+  A.ranges = static_cast<int>(ceil_div(A.packs, A.across * M));
+  const int64_t down = kGradThreads / A.across;
+  // Small chunks where large ones leave the SMs short of blocks.
+  const bool small = self || ceil_div(ceil_div(count, kChunk), down) * A.ranges < E->ctx->sm_count;
+  A.chunks = static_cast<int>(ceil_div(count, small ? kSmallChunk : kChunk));
+  A.chunk_blocks = static_cast<int>(ceil_div(A.chunks, down));
   A.ldo = dout.ld;
   A.ldt = dtable.ld;
   A.parts = E->parts.get();
   A.tickets = E->tickets.as<unsigned>();
   A.err = E->ctx->index_err();
-  const unsigned ranges = static_cast<unsigned>(ceil_div(A.packs, A.across * M));
-  // Without a sort before it the kernel writes the empty rows too; they are
-  // whole rows, so where it takes the columns in ranges they have a launch.
-  unsigned blocks = A.chunk_blocks;
-  if (self && Z.table && ranges == 1) {
-    blocks += share_rows(Z, E->ctx->sm_count * 8, kSelfTokens * 32);
-    A.empty = Z;
-  } else if (self && Z.table) {
-    SPMVB_TRY(launch_empty_rows(Z, tokens, count, E->ctx->sm_count, s));
-  }
+  A.empty_blocks = Z.table ? static_cast<int>(ceil_div(Z.rows, Z.per_block)) : 0;
+  A.empty = Z;
+  const int64_t blocks = static_cast<int64_t>(A.chunk_blocks) * A.ranges + A.empty_blocks;
   if (blocks == 0) return SPMVB_OK;
-  const auto kernel = self ? (accumulate ? grad_rows<T, G, N, true, true> : grad_rows<T, G, N, true, false>)
-                           : (accumulate ? grad_rows<T, G, N, false, true> : grad_rows<T, G, N, false, false>);
-  kernel<<<dim3(blocks, ranges), kGradThreads, 0, s>>>(A, static_cast<const T*>(dout.p), Acc(scale),
-                                                       static_cast<G*>(const_cast<void*>(dtable.p)));
+  if (blocks > INT32_MAX) return fail(SPMVB_ERR_UNSUPPORTED, "too many tokens for one launch");
+  const auto kernel = self    ? (accumulate ? grad_rows<T, G, N, kSmallChunk, true, true> : grad_rows<T, G, N, kSmallChunk, true, false>)
+                      : small ? (accumulate ? grad_rows<T, G, N, kSmallChunk, false, true> : grad_rows<T, G, N, kSmallChunk, false, false>)
+                              : (accumulate ? grad_rows<T, G, N, kChunk, false, true> : grad_rows<T, G, N, kChunk, false, false>);
+  kernel<<<static_cast<unsigned>(blocks), kGradThreads, 0, s>>>(A, static_cast<const T*>(dout.p), Acc(scale),
+                                                                static_cast<G*>(const_cast<void*>(dtable.p)));
   count_launch();
   SPMVB_TRY_CUDA(cudaGetLastError());
   return SPMVB_OK;
@@ -818,9 +914,9 @@ spmvb_status spmvb_embedding_create(spmvb_context ctx, int32_t rows, int32_t wid
     E->width = width;
     E->max_tokens = max_tokens;
     SPMVB_TRY(E->sort.alloc(max_tokens));
+    SPMVB_TRY(E->named.alloc(static_cast<size_t>(ceil_div(rows, 32)) * 4));
     SPMVB_TRY_CUDA(cudaFuncSetAttribute(order_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize, kOrderShared));
-    const size_t chunks = static_cast<size_t>(
-        std::max(ceil_div(max_tokens, chunk_of(false)), ceil_div(std::min(max_tokens, kSelfTokens), chunk_of(true))));
+    const size_t chunks = static_cast<size_t>(ceil_div(max_tokens, kSmallChunk));
     SPMVB_TRY(E->parts.alloc(chunks * 2 * width * 8));
     SPMVB_TRY(E->tickets.alloc(chunks * ceil_div(width, kGradThreads) * 4));
     *out = E.release();
@@ -879,12 +975,15 @@ spmvb_status spmvb_embedding_lookup_grad(spmvb_embedding E, spmvb_dtype dtype, i
     Z.pitch = ld_dtable * static_cast<int64_t>(dtable.elem);
     Z.bytes = E->width * static_cast<int64_t>(dtable.elem);
     Z.rows = E->rows;
+    Z.per_block = kEmptyRows * static_cast<int>(std::min<int64_t>(kMaxEmptyRows / kEmptyRows, std::max<int64_t>(1, 4096 / Z.bytes)));
     Z.wide = access_bytes(dtable.elem, {{dtable.p, dtable.ld}}, E->width) == 16;
     Z.elem = dtable.elem == 2 ? 2 : 4;
   }
   Sorted sorted{};  // no keys: the kernel sorts
   if (count > kSelfTokens || (count > 0 && E->rows >= (1 << 23)))
-    SPMVB_TRY(order_and_clear(E->sort, d_tokens, count, E->rows, Z, E->ctx->sm_count, E->ctx->index_err(), s, &sorted));
+    SPMVB_TRY(order_tokens_by_row(E->sort, d_tokens, count, E->rows, Z.table ? E->named.as<uint32_t>() : nullptr,
+                                  E->ctx->index_err(), s, &sorted));
+  if (sorted.keys) Z.named = E->named.as<uint8_t>();
   // Values of a pack: dout's rows allow one access for them, dtable's 16-byte
   // accesses or one.
   int n = access_bytes(dout.elem, {{dout.p, dout.ld}}, E->width) / static_cast<int>(dout.elem);
