@@ -1,11 +1,13 @@
 // The global 2-norm of many tensors, and their scaling by
 // min(1, max_norm / (norm + eps)) in place.
 //
-// The tensors are cut into pieces of at most kPiece elements. sum_squares
-// sums each block's pieces in fp64, norm_factor adds the blocks' sums in a
-// fixed order and forms the factor, scale_pieces multiplies, and leaves the
-// tensors alone where the factor is 1. The data is read twice and written once, so HBM
-// bounds it.
+// The tensors are cut into pieces of 4 to 16 KB. sum_squares sums each block's
+// pieces in fp64; the last block to finish adds the blocks' sums in their order
+// and forms the factor. scale_pieces multiplies, from the last piece to the
+// first, so that it finds in the L2 what was read last, and leaves the tensors
+// alone where the factor is 1. HBM bounds both: the data is read twice and
+// written once (no cache holds it in between). fp64 costs the bf16 sum nothing
+// yet: its conversions take 0.7 of the reading time.
 #include <cmath>
 #include <iterator>
 #include <vector>
@@ -16,8 +18,8 @@ namespace spmvb {
 namespace {
 
 constexpr int kClipThreads = 256;
-constexpr int kPiece = 16384;
-constexpr int kMaxBlocks = 1184;  // 148 SMs x 8
+constexpr int kClipBlocks = 148 * 6;
+constexpr int64_t kMinPiece = 4096, kMaxPiece = 16384;  // bytes
 
 struct Piece {
   void* p;
@@ -25,15 +27,55 @@ struct Piece {
   int dtype;
 };
 
+// Calls whole(place, word) for the 16-byte words of a piece, four loads ahead,
+// and one(element) for the elements before and after them.
+template <typename T, typename Whole, typename One>
+__device__ __forceinline__ void each_word(const Piece& c, Whole&& whole, One&& one) {
+  constexpr int N = 16 / sizeof(T);
+  T* p = static_cast<T*>(c.p);
+  const int head = min(c.count, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T)));
+  const int words = (c.count - head) / N;
+  uint4* w = reinterpret_cast<uint4*>(p + head) + threadIdx.x;
+  int left = words - static_cast<int>(threadIdx.x);
+  for (; left > 3 * kClipThreads; left -= 4 * kClipThreads, w += 4 * kClipThreads) {
+    const uint4 a = w[0], b = w[kClipThreads], d = w[2 * kClipThreads], e = w[3 * kClipThreads];
+    whole(w, a);
+    whole(w + kClipThreads, b);
+    whole(w + 2 * kClipThreads, d);
+    whole(w + 3 * kClipThreads, e);
+  }
+  for (; left > 0; left -= kClipThreads, w += kClipThreads) whole(w, *w);
+  const int tail = head + words * N;
+  if (static_cast<int>(threadIdx.x) < head) one(p + threadIdx.x);
+  if (tail + static_cast<int>(threadIdx.x) < c.count) one(p + tail + threadIdx.x);
+}
+
+template <typename T>
+__device__ __forceinline__ Pack<T, 16> as_pack(const uint4& v) {
+  Pack<T, 16> p;
+  *reinterpret_cast<uint4*>(&p) = v;
+  return p;
+}
+
 template <typename T>
 __device__ __forceinline__ double piece_squares(const Piece& c) {
-  const T* p = static_cast<const T*>(c.p);
-  double s = 0;
-  for (int i = threadIdx.x; i < c.count; i += kClipThreads) {
-    const double v = static_cast<double>(widen(p[i]));
-    s = fma(v, v, s);
-  }
-  return s;
+  double s0 = 0, s1 = 0;
+  each_word<T>(
+      c,
+      [&](const uint4*, const uint4& v) {
+        const Pack<T, 16> x = as_pack<T>(v);
+#pragma unroll
+        for (int i = 0; i < Pack<T, 16>::N; i += 2) {
+          const double a = static_cast<double>(widen(x.v[i])), b = static_cast<double>(widen(x.v[i + 1]));
+          s0 = fma(a, a, s0);
+          s1 = fma(b, b, s1);
+        }
+      },
+      [&](const T* p) {
+        const double a = static_cast<double>(widen(*p));
+        s0 = fma(a, a, s0);
+      });
+  return s0 + s1;
 }
 
 // Sum over the block, valid in thread 0.
@@ -41,6 +83,7 @@ __device__ __forceinline__ double clip_block_sum(double v) {
   __shared__ double sh[kClipThreads / 32];
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  __syncthreads();
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0;
@@ -49,29 +92,41 @@ __device__ __forceinline__ double clip_block_sum(double v) {
   return v;
 }
 
-__global__ void __launch_bounds__(kClipThreads)
-    sum_squares(const Piece* __restrict__ pieces, int count, double* __restrict__ sums) {
+// Calls f(T{}) for the type of a piece; Only: that of all tensors, or -1.
+template <int Only, typename F>
+__device__ __forceinline__ void with_piece(const Piece& c, F&& f) {
+  const int d = Only >= 0 ? Only : c.dtype;
+  if (d == SPMVB_F32) f(float{});
+  else if (d == SPMVB_F64) f(double{});
+  else if (d == SPMVB_F16) f(__half{});
+  else f(__nv_bfloat16{});
+}
+
+// `ticket` is 0 between calls.
+template <int Only>
+__global__ void __launch_bounds__(kClipThreads, kClipBlocks / 148)
+    sum_squares(const Piece* __restrict__ pieces, int count, double* __restrict__ sums, unsigned* __restrict__ ticket,
+                double max_norm, double eps, float* __restrict__ norm, double* __restrict__ factor) {
+  __shared__ bool last;
   double s = 0;
   for (int c = blockIdx.x; c < count; c += gridDim.x) {
     const Piece q = pieces[c];
-    switch (q.dtype) {
-      case SPMVB_F32: s += piece_squares<float>(q); break;
-      case SPMVB_F64: s += piece_squares<double>(q); break;
-      case SPMVB_F16: s += piece_squares<__half>(q); break;
-      default: s += piece_squares<__nv_bfloat16>(q); break;
-    }
+    with_piece<Only>(q, [&](auto tv) { s += piece_squares<decltype(tv)>(q); });
   }
   s = clip_block_sum(s);
-  if (threadIdx.x == 0) sums[blockIdx.x] = s;
-}
-
-__global__ void __launch_bounds__(kClipThreads)
-    norm_factor(const double* __restrict__ sums, int blocks, double max_norm, double eps, float* __restrict__ norm,
-                double* __restrict__ factor) {
-  double s = 0;
-  for (int i = threadIdx.x; i < blocks; i += kClipThreads) s += sums[i];
+  if (threadIdx.x == 0) {
+    __stcg(sums + blockIdx.x, s);
+    __threadfence();
+    last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  s = 0;
+  for (int i = threadIdx.x; i < gridDim.x; i += kClipThreads) s += __ldcg(sums + i);
   s = clip_block_sum(s);
   if (threadIdx.x == 0) {
+    *ticket = 0u;
     const double n = sqrt(s), f = max_norm / (n + eps);
     *norm = static_cast<float>(n);
     *factor = n + eps > 0 ? (f > 1.0 ? 1.0 : f) : n == n ? 1.0 : n;  // NaN carries on
@@ -81,23 +136,26 @@ __global__ void __launch_bounds__(kClipThreads)
 template <typename T>
 __device__ __forceinline__ void piece_scale(const Piece& c, double factor) {
   using Acc = typename AccOf<T>::type;
-  T* p = static_cast<T*>(c.p);
   const Acc f = static_cast<Acc>(factor);
-  for (int i = threadIdx.x; i < c.count; i += kClipThreads) p[i] = narrow<T, Acc>(widen(p[i]) * f);
+  each_word<T>(
+      c,
+      [&](uint4* to, const uint4& v) {
+        Pack<T, 16> x = as_pack<T>(v);
+#pragma unroll
+        for (int i = 0; i < Pack<T, 16>::N; ++i) x.v[i] = narrow<T, Acc>(widen(x.v[i]) * f);
+        __stcs(to, *reinterpret_cast<const uint4*>(&x));
+      },
+      [&](T* p) { *p = narrow<T, Acc>(widen(*p) * f); });
 }
 
-__global__ void __launch_bounds__(kClipThreads)
+template <int Only>
+__global__ void __launch_bounds__(kClipThreads, kClipBlocks / 148)
     scale_pieces(const Piece* __restrict__ pieces, int count, const double* __restrict__ factor) {
   const double f = *factor;
   if (f == 1.0) return;
-  for (int c = blockIdx.x; c < count; c += gridDim.x) {
+  for (int c = count - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= gridDim.x) {
     const Piece q = pieces[c];
-    switch (q.dtype) {
-      case SPMVB_F32: piece_scale<float>(q, f); break;
-      case SPMVB_F64: piece_scale<double>(q, f); break;
-      case SPMVB_F16: piece_scale<__half>(q, f); break;
-      default: piece_scale<__nv_bfloat16>(q, f); break;
-    }
+    with_piece<Only>(q, [&](auto tv) { piece_scale<decltype(tv)>(q, f); });
   }
 }
 
@@ -106,8 +164,9 @@ __global__ void __launch_bounds__(kClipThreads)
 
 struct spmvb_clip_st {
   int device = 0, pieces = 0, blocks = 0;
+  int only = -1;  // the dtype of all tensors, -1 where they differ
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;  // of the tensors' bytes, ascending
-  spmvb::DevBuf table, sums, factor;
+  spmvb::DevBuf table, sums, factor, ticket;
 };
 
 using namespace spmvb;
@@ -126,9 +185,14 @@ spmvb_status check_norm(spmvb_clip C, const float* d_norm) {
 }
 
 spmvb_status run_norm(spmvb_clip C, double max_norm, double eps, float* d_norm, cudaStream_t s) {
-  sum_squares<<<C->blocks, kClipThreads, 0, s>>>(C->table.as<Piece>(), C->pieces, C->sums.as<double>());
-  norm_factor<<<1, kClipThreads, 0, s>>>(C->sums.as<double>(), C->blocks, max_norm, eps, d_norm, C->factor.as<double>());
-  count_launch(2);
+  const auto kernel = C->only == SPMVB_F32    ? sum_squares<SPMVB_F32>
+                      : C->only == SPMVB_F64  ? sum_squares<SPMVB_F64>
+                      : C->only == SPMVB_F16  ? sum_squares<SPMVB_F16>
+                      : C->only == SPMVB_BF16 ? sum_squares<SPMVB_BF16>
+                                              : sum_squares<-1>;
+  kernel<<<C->blocks, kClipThreads, 0, s>>>(C->table.as<Piece>(), C->pieces, C->sums.as<double>(),
+                                            C->ticket.as<unsigned>(), max_norm, eps, d_norm, C->factor.as<double>());
+  count_launch();
   SPMVB_TRY_CUDA(cudaGetLastError());
   return SPMVB_OK;
 }
@@ -147,18 +211,29 @@ spmvb_status spmvb_clip_create(spmvb_context ctx, int32_t count, void* const* h_
     std::vector<Piece> pieces;
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
     DeviceGuard g(ctx->device);
+    int64_t total = 0;
+    for (int32_t i = 0; i < count; ++i) {
+      if (!any_float(h_dtypes[i])) return fail(SPMVB_ERR_INVALID_ARGUMENT, "tensor " + std::to_string(i) + ": bad dtype");
+      if (h_sizes[i] < 0) return fail(SPMVB_ERR_INVALID_ARGUMENT, "tensor " + std::to_string(i) + ": negative size");
+      total += h_sizes[i] * static_cast<int64_t>(dtype_size(h_dtypes[i]));
+    }
+    // Small pieces where large ones would leave SMs without any.
+    int64_t piece = kMinPiece;
+    while (piece < kMaxPiece && piece * 2 * kClipBlocks <= total) piece *= 2;
     for (int32_t i = 0; i < count; ++i) {
       const std::string name = "tensor " + std::to_string(i);
-      if (!any_float(h_dtypes[i])) return fail(SPMVB_ERR_INVALID_ARGUMENT, name + ": bad dtype");
-      if (h_sizes[i] < 0) return fail(SPMVB_ERR_INVALID_ARGUMENT, name + ": negative size");
       if (h_sizes[i] == 0) continue;
       const size_t es = dtype_size(h_dtypes[i]);
       SPMVB_TRY(check_rows({h_tensors[i], 1, h_sizes[i], h_sizes[i], es, name.c_str()}, ctx->device));
       const auto a = reinterpret_cast<uintptr_t>(h_tensors[i]);
       spans.emplace_back(a, a + h_sizes[i] * es);
-      for (int64_t at = 0; at < h_sizes[i]; at += kPiece)
-        pieces.push_back({static_cast<char*>(h_tensors[i]) + at * es,
-                          static_cast<int>(std::min<int64_t>(kPiece, h_sizes[i] - at)), static_cast<int>(h_dtypes[i])});
+      // Pieces end on 16-byte boundaries, so that only the first can begin off one.
+      for (int64_t at = 0; at < h_sizes[i];) {
+        const int64_t off = static_cast<int64_t>((a + at * es) & 15) / static_cast<int64_t>(es);
+        const int64_t n = std::min<int64_t>(piece / static_cast<int64_t>(es) - off, h_sizes[i] - at);
+        pieces.push_back({static_cast<char*>(h_tensors[i]) + at * es, static_cast<int>(n), static_cast<int>(h_dtypes[i])});
+        at += n;
+      }
       if (pieces.size() > (size_t(1) << 28)) return fail(SPMVB_ERR_UNSUPPORTED, "too many elements");
     }
     std::sort(spans.begin(), spans.end());
@@ -167,10 +242,14 @@ spmvb_status spmvb_clip_create(spmvb_context ctx, int32_t count, void* const* h_
     auto C = std::make_unique<spmvb_clip_st>();
     C->device = ctx->device;
     C->pieces = static_cast<int>(pieces.size());
-    C->blocks = std::max(1, std::min(C->pieces, kMaxBlocks));
+    C->only = count > 0 ? static_cast<int>(h_dtypes[0]) : -1;
+    for (int32_t i = 1; i < count; ++i)
+      if (h_dtypes[i] != h_dtypes[0]) C->only = -1;
+    C->blocks = std::max(1, std::min(C->pieces, kClipBlocks));
     SPMVB_TRY(upload(C->table, pieces.data(), pieces.size() * sizeof(Piece), 16));
     SPMVB_TRY(C->sums.alloc(static_cast<size_t>(C->blocks) * 8));
     SPMVB_TRY(C->factor.alloc(8));
+    SPMVB_TRY(C->ticket.alloc(4));
     C->spans = std::move(spans);
     *out = C.release();
     return SPMVB_OK;
@@ -204,7 +283,12 @@ spmvb_status spmvb_clip_run(spmvb_clip C, double max_norm, double eps, float* d_
   const auto s = static_cast<cudaStream_t>(stream);
   SPMVB_TRY(run_norm(C, max_norm, eps, d_norm, s));
   if (C->pieces == 0) return SPMVB_OK;
-  scale_pieces<<<C->blocks, kClipThreads, 0, s>>>(C->table.as<Piece>(), C->pieces, C->factor.as<double>());
+  const auto kernel = C->only == SPMVB_F32    ? scale_pieces<SPMVB_F32>
+                      : C->only == SPMVB_F64  ? scale_pieces<SPMVB_F64>
+                      : C->only == SPMVB_F16  ? scale_pieces<SPMVB_F16>
+                      : C->only == SPMVB_BF16 ? scale_pieces<SPMVB_BF16>
+                                              : scale_pieces<-1>;
+  kernel<<<C->blocks, kClipThreads, 0, s>>>(C->table.as<Piece>(), C->pieces, C->factor.as<double>());
   count_launch();
   SPMVB_TRY_CUDA(cudaGetLastError());
   return SPMVB_OK;

@@ -270,17 +270,16 @@ class GradClip(_Handle):
             if not t.is_contiguous():
                 raise ValueError(f"tensor {i} must be contiguous")
         n = len(tensors)
-        self._at = [(t, t.data_ptr(), t.numel()) for t in tensors]
+        self._tensors, self._places = tensors, [t.data_ptr() for t in tensors]
         h = C.c_void_p()
-        call("spmvb_clip_create", ctx.handle, n, (C.c_void_p * n)(*[p for _, p, _ in self._at]),
-             (C.c_int64 * n)(*[c for _, _, c in self._at]), (C.c_int * n)(*[_code(t.dtype) for t in tensors]),
+        call("spmvb_clip_create", ctx.handle, n, (C.c_void_p * n)(*self._places),
+             (C.c_int64 * n)(*[t.numel() for t in tensors]), (C.c_int * n)(*[_code(t.dtype) for t in tensors]),
              C.byref(h))
         self.handle, self.ctx = h, ctx
 
     def _check(self, norm) -> int:
-        for t, p, n in self._at:
-            if t.data_ptr() != p or t.numel() != n:
-                raise ValueError("a tensor's storage has been replaced: make a new GradClip")
+        if [t.data_ptr() for t in self._tensors] != self._places:
+            raise ValueError("a tensor's storage has been replaced: make a new GradClip")
         return _flat(norm, FLOAT32, 1, self.ctx.device, "norm")
 
     def norm(self, norm, stream=None) -> None:
