@@ -998,8 +998,8 @@ spmvb_status spmvb_router_dispatch_grad(spmvb_router R, spmvb_dtype dtype, int32
   DeviceGuard g(dev);
   for (const RowSet* r : {&dout, &dX}) SPMVB_TRY(check_rows(*r, dev));
   for (const RowSet* r : {&pos, &dout}) SPMVB_TRY(check_apart(dX, *r));
-  return launch_lookup(dtype, d_position, nullptr, tokens, R->spec.k, out_rows, 1.0, dout, dX, R->ctx->index_err(),
-                       static_cast<cudaStream_t>(stream));
+  return launch_gather_sum(dtype, d_position, nullptr, tokens, R->spec.k, dout, dX, R->ctx->index_err(),
+                           static_cast<cudaStream_t>(stream));
 }
 
 spmvb_status spmvb_router_combine(spmvb_router R, spmvb_dtype dtype, int32_t tokens, int32_t width,
@@ -1015,8 +1015,8 @@ spmvb_status spmvb_router_combine(spmvb_router R, spmvb_dtype dtype, int32_t tok
   DeviceGuard g(dev);
   for (const RowSet* r : {&w, &Y, &out}) SPMVB_TRY(check_rows(*r, dev));
   for (const RowSet* r : {&pos, &w, &Y}) SPMVB_TRY(check_apart(out, *r));
-  return launch_lookup(dtype, d_position, d_weights, tokens, R->spec.k, y_rows, 1.0, Y, out, R->ctx->index_err(),
-                       static_cast<cudaStream_t>(stream));
+  return launch_gather_sum(dtype, d_position, d_weights, tokens, R->spec.k, Y, out, R->ctx->index_err(),
+                           static_cast<cudaStream_t>(stream));
 }
 
 spmvb_status spmvb_router_combine_grad(spmvb_router R, spmvb_dtype dtype, int32_t tokens, int32_t width,

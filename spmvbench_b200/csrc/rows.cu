@@ -10,6 +10,11 @@
 // Each is one pass over its rows: every row is read once and written once,
 // so HBM bounds all of them. Sums over j run in order in fp32 (fp64 for
 // doubles) and are rounded once.
+//
+// Rows are moved in 16-byte words of the row that is written. Where every row
+// begins on such a word (Aligned), the words of the rows read are the same;
+// else a word is put together from the two that hold its bytes, and the
+// elements before the first and after the last whole word are moved alone.
 #include "select.cuh"
 
 namespace spmvb {
@@ -26,162 +31,407 @@ __device__ __forceinline__ int checked(int i, int rows, int* __restrict__ err) {
   return i < 0 ? -1 : i;
 }
 
-// out[t] = scale * sum_j w[t,j] * X[idx[t,j]] (w null: 1). blockDim.x threads
-// share a row, blockDim.y rows share a block.
-template <typename T, int VB, bool Weighted>
+// 16 bytes from an address that is aligned to its elements alone. Only words
+// that hold one of the bytes are read.
+template <typename T, bool Aligned>
+__device__ __forceinline__ Pack<T, 16> ld_word(const T* p) {
+  Pack<T, 16> r;
+  if constexpr (Aligned) {
+    *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
+  } else {
+    const auto a = reinterpret_cast<uintptr_t>(p);
+    const unsigned off = static_cast<unsigned>(a & 15u);
+    const uint4* w = reinterpret_cast<const uint4*>(a - off);
+    const uint4 x = __ldg(w), y = off ? __ldg(w + 1) : make_uint4(0, 0, 0, 0);
+    // Words off / 4 .. off / 4 + 4 of the eight, then the bytes within.
+    uint32_t v0 = x.x, v1 = x.y, v2 = x.z, v3 = x.w, v4 = y.x;
+    if (off & 8u) {
+      v0 = x.z; v1 = x.w; v2 = y.x; v3 = y.y; v4 = y.z;
+    }
+    if (off & 4u) {
+      v0 = v1; v1 = v2; v2 = v3; v3 = v4; v4 = off & 8u ? y.w : y.y;
+    }
+    const unsigned bits = (off & 3u) * 8u;
+    uint4 o = make_uint4(v0, v1, v2, v3);
+    if constexpr (sizeof(T) == 2)
+      o = make_uint4(__funnelshift_r(v0, v1, bits), __funnelshift_r(v1, v2, bits), __funnelshift_r(v2, v3, bits),
+                     __funnelshift_r(v3, v4, bits));
+    *reinterpret_cast<uint4*>(&r) = o;
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void st_word(T* p, const Pack<T, 16>& v) {
+  __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+}
+
+// The words of a row that is written: elements first .. first + 16 / size - 1
+// of word v. Unaligned rows have a word 0 of the elements before the first
+// 16-byte boundary and a last one of those after the last: `count` < N.
+template <typename T, bool Aligned>
+struct Words {
+  static constexpr int N = 16 / sizeof(T);
+  int head, width;
+  __device__ __forceinline__ Words(const T* row, int w)
+      : head(Aligned ? 0 : min(w, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(T)))),
+        width(w) {}
+  __device__ __forceinline__ int first(int v) const { return Aligned ? v * N : v == 0 ? 0 : head + (v - 1) * N; }
+  __device__ __forceinline__ int count(int v) const {
+    if constexpr (Aligned) return N;
+    return v == 0 ? head : min(N, width - first(v));  // <= 0: past the end
+  }
+};
+// Words of a row of any alignment, at most.
+inline int words_of(int width, size_t elem, bool aligned) {
+  const int n = static_cast<int>(16 / elem);
+  return aligned ? width / n : (width + n - 1) / n + 1;
+}
+
+// out[t] = scale * X[idx[t]]. blockDim.x threads share a row and take Ahead
+// words of it at a time.
+constexpr int kAhead = 4;
+template <typename T, bool Aligned>
+__global__ void __launch_bounds__(kRowThreads)
+    copy_rows(const int* __restrict__ idx, int count, int rows, typename AccOf<T>::type scale, const T* __restrict__ X,
+              int64_t ldx, T* __restrict__ out, int64_t ldo, int width, int words, int* __restrict__ err) {
+  using Acc = typename AccOf<T>::type;
+  constexpr int N = 16 / sizeof(T);
+  const int t = blockIdx.x * blockDim.y + threadIdx.y;
+  if (t >= count) return;
+  const int r = checked(__ldg(idx + t), rows, err);
+  T* to = out + t * ldo;
+  const T* from = X + max(r, 0) * ldx;
+  const Words<T, Aligned> W(to, width);
+  for (int v0 = threadIdx.x; v0 < words; v0 += blockDim.x * kAhead) {
+    Pack<T, 16> p[kAhead];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int v = v0 + q * blockDim.x;
+      if (v < words && r >= 0 && W.count(v) == N) p[q] = ld_word<T, Aligned>(from + W.first(v));
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int v = v0 + q * blockDim.x;
+      if (v >= words) continue;
+      const int e = W.first(v), n = W.count(v);
+      if (n == N) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[q].v[i] = r >= 0 ? narrow<T, Acc>(widen(p[q].v[i]) * scale) : narrow<T, Acc>(0);
+        st_word(to + e, p[q]);
+      } else {
+        for (int i = 0; i < n; ++i) to[e + i] = r >= 0 ? narrow<T, Acc>(widen(__ldg(from + e + i)) * scale) : narrow<T, Acc>(0);
+      }
+    }
+  }
+}
+
+// out[t] = sum_j w[t,j] * X[idx[t,j]], kAhead rows loaded at a time.
+template <typename T, bool Aligned, bool Weighted>
 __global__ void __launch_bounds__(kRowThreads)
     gather_sum(const int* __restrict__ idx, const float* __restrict__ w, int count, int k, int rows,
-               typename AccOf<T>::type scale, const T* __restrict__ X, int64_t ldx, T* __restrict__ out, int64_t ldo,
-               int packs, int* __restrict__ err) {
-  using Acc = typename AccOf<T>::type;
-  constexpr int N = Pack<T, VB>::N;
+               const T* __restrict__ X, int64_t ldx, T* __restrict__ out, int64_t ldo, int width, int words,
+               int* __restrict__ err) {
+  constexpr int N = 16 / sizeof(T);
   const int t = blockIdx.x * blockDim.y + threadIdx.y;
   if (t >= count) return;
   const int64_t e0 = static_cast<int64_t>(t) * k;
-  for (int v = threadIdx.x; v < packs; v += blockDim.x) {
-    Acc sum[N] = {};
-    for (int j = 0; j < k; ++j) {
-      const int r = checked(__ldg(idx + e0 + j), rows, err);
-      if (r < 0) continue;
-      const Pack<T, VB> p = ld_pack<T, VB>(X + r * ldx + static_cast<int64_t>(v) * N);
-      const Acc f = Weighted ? static_cast<Acc>(__ldg(w + e0 + j)) : Acc(1);
+  T* to = out + t * ldo;
+  const Words<T, Aligned> W(to, width);
+  for (int v = threadIdx.x; v < words; v += blockDim.x) {
+    const int e = W.first(v), n = W.count(v);
+    if (n == N) {
+      float sum[N] = {};
+      for (int j0 = 0; j0 < k; j0 += kAhead) {
+        Pack<T, 16> p[kAhead];
+        int r[kAhead];
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum[i] += f * widen(p.v[i]);
+        for (int q = 0; q < kAhead; ++q) r[q] = j0 + q < k ? __ldg(idx + e0 + j0 + q) : -1;
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q)
+          if (static_cast<unsigned>(r[q]) < static_cast<unsigned>(rows)) p[q] = ld_word<T, Aligned>(X + r[q] * ldx + e);
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+          if (checked(r[q], rows, err) < 0) continue;
+          const float f = Weighted ? __ldg(w + e0 + j0 + q) : 1.f;
+#pragma unroll
+          for (int i = 0; i < N; ++i) sum[i] += f * widen(p[q].v[i]);
+        }
+      }
+      Pack<T, 16> o;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o.v[i] = narrow<T, float>(sum[i]);
+      st_word(to + e, o);
+    } else {
+      for (int i = 0; i < n; ++i) {
+        float sum = 0.f;
+        for (int j = 0; j < k; ++j) {
+          const int r = checked(__ldg(idx + e0 + j), rows, err);
+          if (r >= 0) sum += (Weighted ? __ldg(w + e0 + j) : 1.f) * widen(__ldg(X + r * ldx + e + i));
+        }
+        to[e + i] = narrow<T, float>(sum);
+      }
     }
-    Pack<T, VB> o;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o.v[i] = narrow<T, Acc>(sum[i] * scale);
-    st_pack_stream<T, VB>(out + t * ldo + static_cast<int64_t>(v) * N, o);
   }
 }
 
-// out[pos[t,j]] = X[t]: the row is read once and written to each of its places.
-template <typename T, int VB>
+// out[pos[t,j]] = X[t]. Aligned rows are read once and written to each of their
+// places; others are read again for each place (from the L1), as the words
+// that are written lie differently in each.
+template <typename T, bool Aligned>
 __global__ void __launch_bounds__(kRowThreads)
     scatter_rows(const int* __restrict__ pos, int count, int k, const T* __restrict__ X, int64_t ldx, int rows,
-                 T* __restrict__ out, int64_t ldo, int packs, int* __restrict__ err) {
-  constexpr int N = Pack<T, VB>::N;
+                 T* __restrict__ out, int64_t ldo, int width, int words, int* __restrict__ err) {
+  constexpr int N = 16 / sizeof(T), Two = 2;
   const int t = blockIdx.x * blockDim.y + threadIdx.y;
   if (t >= count) return;
   const int64_t e0 = static_cast<int64_t>(t) * k;
-  for (int v = threadIdx.x; v < packs; v += blockDim.x) {
-    const Pack<T, VB> p = ld_pack_stream<T, VB>(X + t * ldx + static_cast<int64_t>(v) * N);
+  const T* from = X + t * ldx;
+  if constexpr (Aligned) {
+    for (int v = threadIdx.x; v < words; v += blockDim.x * Two) {
+      Pack<T, 16> p[Two];
+#pragma unroll
+      for (int q = 0; q < Two; ++q)
+        if (v + q * blockDim.x < words) p[q] = ld_word<T, true>(from + static_cast<int64_t>(v + q * blockDim.x) * N);
+#pragma unroll 4
+      for (int j = 0; j < k; ++j) {
+        const int r = checked(__ldg(pos + e0 + j), rows, err);
+        if (r < 0) continue;
+#pragma unroll
+        for (int q = 0; q < Two; ++q)
+          if (v + q * blockDim.x < words) st_word(out + r * ldo + static_cast<int64_t>(v + q * blockDim.x) * N, p[q]);
+      }
+    }
+  } else {
     for (int j = 0; j < k; ++j) {
       const int r = checked(__ldg(pos + e0 + j), rows, err);
-      if (r >= 0) st_pack_stream<T, VB>(out + r * ldo + static_cast<int64_t>(v) * N, p);
+      if (r < 0) continue;
+      T* to = out + r * ldo;
+      const Words<T, false> W(to, width);
+#pragma unroll 2
+      for (int v = threadIdx.x; v < words; v += blockDim.x) {
+        const int e = W.first(v), n = W.count(v);
+        if (n == N)
+          st_word(to + e, ld_word<T, false>(from + e));
+        else
+          for (int i = 0; i < n; ++i) to[e + i] = __ldg(from + e + i);
+      }
     }
   }
 }
 
-// One block per token: dout[t] is held while the token's rows of Y pass by;
-// the inner products are summed over each thread's columns, then the warp,
-// then the warps in order.
-template <typename T, int VB>
+// One block per token: dout[t] is held (Held words a thread) while the token's
+// rows of Y pass by, two at a time; the inner products are summed over each
+// word in a tree, each thread's words, then the warp, then the warps in order.
+constexpr int kHeld = 2;
+template <typename T>
+__device__ __forceinline__ float word_dot(const Pack<T, 16>& a, const Pack<T, 16>& b) {
+  constexpr int N = 16 / sizeof(T);
+  float x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = widen(a.v[i]) * widen(b.v[i]);
+#pragma unroll
+  for (int s = N / 2; s > 0; s /= 2)
+#pragma unroll
+    for (int i = 0; i < s; ++i) x[i] += x[i + s];
+  return x[0];
+}
+template <typename T>
+__device__ __forceinline__ Pack<T, 16> scaled(const Pack<T, 16>& a, float f) {
+  Pack<T, 16> o;
+#pragma unroll
+  for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) o.v[i] = narrow<T, float>(f * widen(a.v[i]));
+  return o;
+}
+
+template <typename T, bool Aligned>
 __global__ void __launch_bounds__(kRowThreads)
     combine_grad_rows(const int* __restrict__ pos, const float* __restrict__ w, int k, int rows,
                       const T* __restrict__ Y, int64_t ldy, const T* __restrict__ dout, int64_t ldd,
-                      T* __restrict__ dY, int64_t lddy, float* __restrict__ dw, int packs, int* __restrict__ err) {
-  constexpr int N = Pack<T, VB>::N;
+                      T* __restrict__ dY, int64_t lddy, float* __restrict__ dw, int width, int words,
+                      int* __restrict__ err) {
+  constexpr int N = 16 / sizeof(T), Pair = 2;
   __shared__ float part[32][kRowThreads / 32];
+  __shared__ int place[32];
+  __shared__ float weight[32];
   const int64_t t = blockIdx.x;
   const int64_t e0 = t * k;
-  const int warps = blockDim.x >> 5;
-  for (int j = 0; j < k; ++j) {
-    const int r = checked(__ldg(pos + e0 + j), rows, err);
-    float dot = 0.f;
-    if (r >= 0) {
-      const float f = __ldg(w + e0 + j);
-      for (int v = threadIdx.x; v < packs; v += blockDim.x) {
-        const int64_t c = static_cast<int64_t>(v) * N;
-        const Pack<T, VB> d = ld_pack<T, VB>(dout + t * ldd + c);
-        const Pack<T, VB> y = ld_pack_stream<T, VB>(Y + r * ldy + c);
-        Pack<T, VB> o;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float g = static_cast<float>(widen(d.v[i]));
-          dot += g * static_cast<float>(widen(y.v[i]));
-          o.v[i] = narrow<T, typename AccOf<T>::type>(f * g);
-        }
-        st_pack_stream<T, VB>(dY + r * lddy + c, o);
-      }
-    }
+  const int warps = blockDim.x >> 5, wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (static_cast<int>(threadIdx.x) < k) {
+    place[threadIdx.x] = checked(__ldg(pos + e0 + threadIdx.x), rows, err);
+    weight[threadIdx.x] = __ldg(w + e0 + threadIdx.x);
+  }
+  for (int i = threadIdx.x; i < k * warps; i += blockDim.x) part[i / warps][i % warps] = 0.f;
+  __syncthreads();
+  const T* d = dout + t * ldd;
+  const auto add_up = [&](int j, float dot) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    if ((threadIdx.x & 31) == 0) part[j][threadIdx.x >> 5] = dot;
+    if (lane == 0) part[j][wid] += dot;
+  };
+  if constexpr (Aligned) {
+    // A thread's words v0, v0 + blockDim.x; all threads make the same turns.
+    for (int b = 0; b < words; b += blockDim.x * kHeld) {
+      const int v0 = b + threadIdx.x;
+      Pack<T, 16> held[kHeld];
+#pragma unroll
+      for (int q = 0; q < kHeld; ++q)
+        if (v0 + q * blockDim.x < words) held[q] = ld_word<T, true>(d + static_cast<int64_t>(v0 + q * blockDim.x) * N);
+      for (int j0 = 0; j0 < k; j0 += Pair) {
+        Pack<T, 16> y[Pair][kHeld];
+#pragma unroll
+        for (int u = 0; u < Pair; ++u) {
+          const int r = j0 + u < k ? place[j0 + u] : -1;
+#pragma unroll
+          for (int q = 0; q < kHeld; ++q)
+            if (r >= 0 && v0 + q * blockDim.x < words)
+              y[u][q] = ld_word<T, true>(Y + r * ldy + static_cast<int64_t>(v0 + q * blockDim.x) * N);
+        }
+#pragma unroll
+        for (int u = 0; u < Pair; ++u) {
+          const int r = j0 + u < k ? place[j0 + u] : -1;
+          if (r < 0) continue;
+          float dot = 0.f;
+#pragma unroll
+          for (int q = 0; q < kHeld; ++q) {
+            if (v0 + q * blockDim.x >= words) continue;
+            dot += word_dot<T>(held[q], y[u][q]);
+            st_word(dY + r * lddy + static_cast<int64_t>(v0 + q * blockDim.x) * N, scaled<T>(held[q], weight[j0 + u]));
+          }
+          add_up(j0 + u, dot);
+        }
+      }
+    }
+  } else {
+    for (int j = 0; j < k; ++j) {
+      const int r = place[j];
+      if (r < 0) continue;
+      T* to = dY + r * lddy;
+      const T* y = Y + r * ldy;
+      const Words<T, false> W(to, width);
+      float dot = 0.f;
+#pragma unroll 2
+      for (int v = threadIdx.x; v < words; v += blockDim.x) {
+        const int e = W.first(v), n = W.count(v);
+        if (n == N) {
+          const Pack<T, 16> a = ld_word<T, false>(d + e);
+          dot += word_dot<T>(a, ld_word<T, false>(y + e));
+          st_word(to + e, scaled<T>(a, weight[j]));
+        } else {
+          for (int i = 0; i < n; ++i) {
+            const float g = widen(__ldg(d + e + i));
+            dot += g * widen(__ldg(y + e + i));
+            to[e + i] = narrow<T, float>(weight[j] * g);
+          }
+        }
+      }
+      add_up(j, dot);
+    }
   }
   __syncthreads();
-  if (threadIdx.x < k) {
+  if (static_cast<int>(threadIdx.x) < k) {
     float sum = 0.f;
     for (int i = 0; i < warps; ++i) sum += part[threadIdx.x][i];
     dw[e0 + threadIdx.x] = sum;
   }
 }
 
-// Threads of a block: x along the row (a power of two of at most 256), y rows.
-dim3 row_block(int packs) {
-  int x = 1;
-  while (x < packs && x < kRowThreads) x *= 2;
-  return dim3(x, kRowThreads / x);
+// Threads along a row for `words` words, `each` to a thread: a power of two,
+// 256 at most.
+int across(int words, int each, int least) {
+  int x = least;
+  while (x * each < words && x < kRowThreads) x *= 2;
+  return x;
+}
+
+template <bool F64, typename F>
+spmvb_status with_rows(spmvb_dtype d, bool aligned, F&& f) {
+  const auto by = [&](auto tv) -> spmvb_status {
+    return aligned ? f(tv, std::true_type{}) : f(tv, std::false_type{});
+  };
+  switch (d) {
+    case SPMVB_F32: return by(float{});
+    case SPMVB_F16: return by(__half{});
+    case SPMVB_BF16: return by(__nv_bfloat16{});
+    case SPMVB_F64:
+      if constexpr (F64) return by(double{});
+      break;
+  }
+  return fail(SPMVB_ERR_INVALID_ARGUMENT, "bad dtype");
+}
+
+spmvb_status launched() {
+  count_launch();
+  SPMVB_TRY_CUDA(cudaGetLastError());
+  return SPMVB_OK;
+}
+
+template <typename T>
+T* rows_at(const RowSet& r) {
+  return static_cast<T*>(const_cast<void*>(r.p));
 }
 
 }  // namespace
 
-spmvb_status launch_lookup(spmvb_dtype dtype, const int* idx, const float* w, int count, int k, int rows, double scale,
-                           const RowSet& X, const RowSet& out, int* err, cudaStream_t s) {
+spmvb_status launch_lookup(spmvb_dtype dtype, const int* idx, int count, double scale, const RowSet& X,
+                           const RowSet& out, int* err, cudaStream_t s) {
   if (count == 0) return SPMVB_OK;
-  const int vb = access_bytes(X.elem, {{X.p, X.ld}, {out.p, out.ld}}, X.width);
-  return with_type<true>(dtype, vb, [&](auto tv, auto vbc) -> spmvb_status {
+  const bool aligned = access_bytes(X.elem, {{X.p, X.ld}, {out.p, out.ld}}, X.width) == 16;
+  return with_rows<true>(dtype, aligned, [&](auto tv, auto al) -> spmvb_status {
     using T = decltype(tv);
-    using Acc = typename AccOf<T>::type;
-    constexpr int VB = decltype(vbc)::value;
-    const int packs = static_cast<int>(X.width / Pack<T, VB>::N);
-    const dim3 block = row_block(packs);
-    const int grid = static_cast<int>(ceil_div(count, block.y));
-    const T* x = static_cast<const T*>(X.p);
-    T* o = static_cast<T*>(const_cast<void*>(out.p));
-    if (w)
-      gather_sum<T, VB, true><<<grid, block, 0, s>>>(idx, w, count, k, rows, Acc(scale), x, X.ld, o, out.ld, packs, err);
-    else
-      gather_sum<T, VB, false><<<grid, block, 0, s>>>(idx, w, count, k, rows, Acc(scale), x, X.ld, o, out.ld, packs, err);
-    count_launch();
-    SPMVB_TRY_CUDA(cudaGetLastError());
-    return SPMVB_OK;
+    constexpr bool Aligned = decltype(al)::value;
+    const int width = static_cast<int>(X.width), words = words_of(width, sizeof(T), Aligned);
+    const int x = across(words, kAhead, 1), y = kRowThreads / x;
+    copy_rows<T, Aligned><<<static_cast<int>(ceil_div(count, y)), dim3(x, y), 0, s>>>(
+        idx, count, static_cast<int>(X.rows), static_cast<typename AccOf<T>::type>(scale), rows_at<const T>(X), X.ld,
+        rows_at<T>(out), out.ld, width, words, err);
+    return launched();
+  });
+}
+
+spmvb_status launch_gather_sum(spmvb_dtype dtype, const int* idx, const float* w, int count, int k, const RowSet& X,
+                               const RowSet& out, int* err, cudaStream_t s) {
+  if (count == 0) return SPMVB_OK;
+  const bool aligned = access_bytes(X.elem, {{X.p, X.ld}, {out.p, out.ld}}, X.width) == 16;
+  return with_rows<false>(dtype, aligned, [&](auto tv, auto al) -> spmvb_status {
+    using T = decltype(tv);
+    constexpr bool Aligned = decltype(al)::value;
+    const int width = static_cast<int>(X.width), words = words_of(width, sizeof(T), Aligned);
+    const int x = across(words, 1, 1), y = kRowThreads / x;
+    const auto kernel = w ? gather_sum<T, Aligned, true> : gather_sum<T, Aligned, false>;
+    kernel<<<static_cast<int>(ceil_div(count, y)), dim3(x, y), 0, s>>>(idx, w, count, k, static_cast<int>(X.rows),
+                                                                      rows_at<const T>(X), X.ld, rows_at<T>(out), out.ld,
+                                                                      width, words, err);
+    return launched();
   });
 }
 
 spmvb_status launch_dispatch(spmvb_dtype dtype, const int* pos, int count, int k, const RowSet& X, const RowSet& out,
                              int* err, cudaStream_t s) {
   if (count == 0) return SPMVB_OK;
-  const int vb = access_bytes(X.elem, {{X.p, X.ld}, {out.p, out.ld}}, X.width);
-  return with_type<false>(dtype, vb, [&](auto tv, auto vbc) -> spmvb_status {
+  const bool aligned = access_bytes(X.elem, {{X.p, X.ld}, {out.p, out.ld}}, X.width) == 16;
+  return with_rows<false>(dtype, aligned, [&](auto tv, auto al) -> spmvb_status {
     using T = decltype(tv);
-    constexpr int VB = decltype(vbc)::value;
-    const int packs = static_cast<int>(X.width / Pack<T, VB>::N);
-    const dim3 block = row_block(packs);
-    scatter_rows<T, VB><<<static_cast<int>(ceil_div(count, block.y)), block, 0, s>>>(
-        pos, count, k, static_cast<const T*>(X.p), X.ld, static_cast<int>(out.rows),
-        static_cast<T*>(const_cast<void*>(out.p)), out.ld, packs, err);
-    count_launch();
-    SPMVB_TRY_CUDA(cudaGetLastError());
-    return SPMVB_OK;
+    constexpr bool Aligned = decltype(al)::value;
+    const int width = static_cast<int>(X.width), words = words_of(width, sizeof(T), Aligned);
+    const int x = across(words, Aligned ? 2 : 1, 1), y = kRowThreads / x;
+    scatter_rows<T, Aligned><<<static_cast<int>(ceil_div(count, y)), dim3(x, y), 0, s>>>(
+        pos, count, k, rows_at<const T>(X), X.ld, static_cast<int>(out.rows), rows_at<T>(out), out.ld, width, words, err);
+    return launched();
   });
 }
 
 spmvb_status launch_combine_grad(spmvb_dtype dtype, const int* pos, const float* w, int count, int k, const RowSet& Y,
                                  const RowSet& dout, const RowSet& dY, float* dw, int* err, cudaStream_t s) {
   if (count == 0) return SPMVB_OK;
-  const int vb = access_bytes(Y.elem, {{Y.p, Y.ld}, {dout.p, dout.ld}, {dY.p, dY.ld}}, Y.width);
-  return with_type<false>(dtype, vb, [&](auto tv, auto vbc) -> spmvb_status {
+  const bool aligned = access_bytes(Y.elem, {{Y.p, Y.ld}, {dout.p, dout.ld}, {dY.p, dY.ld}}, Y.width) == 16;
+  return with_rows<false>(dtype, aligned, [&](auto tv, auto al) -> spmvb_status {
     using T = decltype(tv);
-    constexpr int VB = decltype(vbc)::value;
-    const int packs = static_cast<int>(Y.width / Pack<T, VB>::N);
-    const int threads = std::max<int>(32, static_cast<int>(row_block(packs).x));
-    combine_grad_rows<T, VB><<<count, threads, 0, s>>>(
-        pos, w, k, static_cast<int>(Y.rows), static_cast<const T*>(Y.p), Y.ld, static_cast<const T*>(dout.p), dout.ld,
-        static_cast<T*>(const_cast<void*>(dY.p)), dY.ld, dw, packs, err);
-    count_launch();
-    SPMVB_TRY_CUDA(cudaGetLastError());
-    return SPMVB_OK;
+    constexpr bool Aligned = decltype(al)::value;
+    const int width = static_cast<int>(Y.width), words = words_of(width, sizeof(T), Aligned);
+    combine_grad_rows<T, Aligned><<<count, across(words, Aligned ? kHeld : 1, 32), 0, s>>>(
+        pos, w, k, static_cast<int>(Y.rows), rows_at<const T>(Y), Y.ld, rows_at<const T>(dout), dout.ld,
+        rows_at<T>(dY), dY.ld, dw, width, words, err);
+    return launched();
   });
 }
 

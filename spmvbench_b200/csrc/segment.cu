@@ -948,8 +948,7 @@ spmvb_status spmvb_embedding_lookup(spmvb_embedding E, spmvb_dtype dtype, int32_
   DeviceGuard g(dev);
   for (const RowSet* r : {&idx, &table, &out}) SPMVB_TRY(check_rows(*r, dev));
   for (const RowSet* r : {&idx, &table}) SPMVB_TRY(check_apart(out, *r));
-  return launch_lookup(dtype, d_tokens, nullptr, count, 1, E->rows, scale, table, out, E->ctx->index_err(),
-                       static_cast<cudaStream_t>(stream));
+  return launch_lookup(dtype, d_tokens, count, scale, table, out, E->ctx->index_err(), static_cast<cudaStream_t>(stream));
 }
 
 spmvb_status spmvb_embedding_lookup_grad(spmvb_embedding E, spmvb_dtype dtype, int32_t count, const int32_t* d_tokens,

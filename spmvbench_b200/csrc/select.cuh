@@ -66,14 +66,6 @@ __device__ __forceinline__ void st_pack_stream(T* p, const Pack<T, VB>& v) {
   using Raw = typename RawOf<VB>::type;
   __stcs(reinterpret_cast<Raw*>(p), *reinterpret_cast<const Raw*>(&v));
 }
-template <typename T, int VB>
-__device__ __forceinline__ Pack<T, VB> zero_pack() {
-  Pack<T, VB> r;
-#pragma unroll
-  for (int i = 0; i < Pack<T, VB>::N; ++i) r.v[i] = narrow<T, typename AccOf<T>::type>(0);
-  return r;
-}
-
 // The widest access that every one of a call's row sets allows: base
 // addresses, row strides and the row length in bytes are multiples of it.
 inline int access_bytes(size_t elem, std::initializer_list<std::pair<const void*, int64_t>> sets, int64_t width) {
@@ -118,32 +110,6 @@ inline spmvb_status check_apart(const RowSet& out, const RowSet& in) {
 inline bool half_or_float(spmvb_dtype d) { return d == SPMVB_F32 || d == SPMVB_F16 || d == SPMVB_BF16; }
 inline bool any_float(spmvb_dtype d) { return half_or_float(d) || d == SPMVB_F64; }
 
-// Calls f(T{}, std::integral_constant<int, VB>{}) for the value type and the
-// access width.
-template <typename T, typename F>
-spmvb_status with_access(int vb, F&& f) {
-  using std::integral_constant;
-  if (vb == 16) return f(T{}, integral_constant<int, 16>{});
-  if (vb == 8) return f(T{}, integral_constant<int, 8>{});
-  if constexpr (sizeof(T) <= 4)
-    if (vb == 4) return f(T{}, integral_constant<int, 4>{});
-  if constexpr (sizeof(T) <= 2)
-    if (vb == 2) return f(T{}, integral_constant<int, 2>{});
-  return fail(SPMVB_ERR_INVALID_ARGUMENT, "row not aligned to its elements");
-}
-template <bool F64, typename F>
-spmvb_status with_type(spmvb_dtype d, int vb, F&& f) {
-  switch (d) {
-    case SPMVB_F32: return with_access<float>(vb, f);
-    case SPMVB_F64:
-      if constexpr (F64) return with_access<double>(vb, f);
-      break;
-    case SPMVB_F16: return with_access<__half>(vb, f);
-    case SPMVB_BF16: return with_access<__nv_bfloat16>(vb, f);
-  }
-  return fail(SPMVB_ERR_INVALID_ARGUMENT, "bad dtype");
-}
-
 // Runs a handle's construction; a failed host allocation becomes a status.
 template <typename F>
 spmvb_status constructed(F&& f) {
@@ -157,9 +123,12 @@ spmvb_status constructed(F&& f) {
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- row products (rows.cu) ------------------------------------------------------
-// out[t] = scale * sum_j w[t,j] * X[idx[t,j]], j < k (w null: 1).
-spmvb_status launch_lookup(spmvb_dtype dtype, const int* idx, const float* w, int count, int k, int rows, double scale,
-                           const RowSet& X, const RowSet& out, int* err, cudaStream_t s);
+// out[t] = scale * X[idx[t]].
+spmvb_status launch_lookup(spmvb_dtype dtype, const int* idx, int count, double scale, const RowSet& X,
+                           const RowSet& out, int* err, cudaStream_t s);
+// out[t] = sum_j w[t,j] * X[idx[t,j]], j < k (w null: 1).
+spmvb_status launch_gather_sum(spmvb_dtype dtype, const int* idx, const float* w, int count, int k, const RowSet& X,
+                               const RowSet& out, int* err, cudaStream_t s);
 // out[pos[t,j]] = X[t].
 spmvb_status launch_dispatch(spmvb_dtype dtype, const int* pos, int count, int k, const RowSet& X, const RowSet& out,
                              int* err, cudaStream_t s);
