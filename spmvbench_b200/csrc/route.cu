@@ -632,86 +632,111 @@ __global__ void __launch_bounds__(kRouteThreads, EPL > 8 ? 2 : 4)
 //   renormalised      scale * p_j * (dw_j - g), times 1 - s_j under the sigmoid
 //   sigmoid           scale * s_j * (1 - s_j) * dw_j
 //   softmax           scale * p_e * ([e chosen] dw_e - g) for every expert
-template <typename T, int EPL>
+//
+// A warp a row. The row is written in words of VB bytes as if nothing were
+// chosen; lane j then writes the j-th choice's own value, with those of equal
+// choices added.
+template <typename T, int VB>
 __global__ void __launch_bounds__(kRouteThreads)
     route_grad_rows(spmvb_router_spec S, const T* __restrict__ logits, int64_t ld, int tokens,
                     const int* __restrict__ indices, const float* __restrict__ dweights, T* __restrict__ dlogits,
                     int64_t ldd, int* __restrict__ err) {
+  constexpr int N = VB / sizeof(T);
   const int lane = threadIdx.x & 31, w0 = blockIdx.x * (kRouteThreads / 32) + (threadIdx.x >> 5);
   const bool real = w0 < tokens;  // a warp past the last token repeats it and writes nothing
   const int64_t t = real ? w0 : tokens - 1;
-  const int E = S.experts, k = S.k;
+  const int k = S.k, words = S.experts / N;
+  const bool softmax = S.score == SPMVB_SOFTMAX;
   const T* row = logits + t * ld;
-  int e = -1;
-  float dw = 0.f, le = -INFINITY;
-  if (lane < k) {
-    e = indices[static_cast<int64_t>(t) * k + lane];
-    if (e >= E) *err = 1;
-    if (e < 0 || e >= E) e = -1;
-    if (e >= 0) {
-      dw = dweights[static_cast<int64_t>(t) * k + lane] * S.scale;
-      le = static_cast<float>(widen(row[e]));
+  T* to = dlogits + t * ldd;
+  const int loaded = lane < k ? __ldg(indices + t * k + lane) : -1;
+  // Zeros need not wait for the loads.
+  if (!softmax && real)
+    for (int v = lane; v < words; v += 32) {
+      Pack<T, VB> o;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o.v[i] = narrow<T, float>(0.f);
+      st_pack_stream<T, VB>(to + v * N, o);
     }
-  }
-  float d = 0.f, g[EPL];
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) g[i] = 0.f;
-  float l[EPL], top = -INFINITY;
+  int e = loaded;
+  if (e >= S.experts) *err = 1;
+  if (e < 0 || e >= S.experts) e = -1;
+  const float dw = e >= 0 ? dweights[t * k + lane] * S.scale : 0.f;
+  const float le = e >= 0 ? static_cast<float>(widen(row[e])) : -INFINITY;
+  float d, top = -INFINITY, inv = 0.f, all = 0.f;
   bool poison = false;
-  if (S.score == SPMVB_SOFTMAX) {
+  if (softmax) {
+    float sum = 0.f;
+    for (int v = lane; v < words; v += 32) {
+      const Pack<T, VB> p = ld_pack<T, VB>(row + v * N);
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int x = lane * EPL + i;
-      l[i] = x < E ? static_cast<float>(widen(row[x])) : -INFINITY;
-      poison |= isnan(l[i]) || l[i] == INFINITY;
-      top = fmaxf(top, l[i]);
+      for (int i = 0; i < N; ++i) {
+        const float l = widen(p.v[i]);
+        poison |= !(l < INFINITY);
+        top = fmaxf(top, l);
+      }
     }
     poison = __any_sync(kAll, poison);
+    if (!S.renormalise) {
+      top = warp_max(top);
+      for (int v = lane; v < words; v += 32) {
+        const Pack<T, VB> p = ld_pack<T, VB>(row + v * N);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float l = widen(p.v[i]);
+          sum += l > -INFINITY ? expf(l - top) : 0.f;
+        }
+      }
+      sum = warp_sum(sum);
+      inv = sum > 0.f ? 1.f / sum : 0.f;
+    }
   }
   if (S.renormalise) {
     float m = warp_max(le);
-    if (S.score == SPMVB_SIGMOID) m = fminf(m, 0.f);
-    float s = 0.f, rest = 1.f;
-    if (e >= 0) {
-      if (S.score == SPMVB_SOFTMAX) {
-        s = expf(le - m);
-      } else {
-        s = le > 0 ? 1.f / (1.f + expf(-le)) : expf(le - m) / (1.f + expf(le));
-        rest = 1.f / (1.f + expf(le));
-      }
-    }
-    const float sum = warp_sum(s);
-    const float p = sum > 0 ? s / sum : 0.f;
-    d = p * (dw - warp_sum(p * dw)) * rest;
-  } else if (S.score == SPMVB_SIGMOID) {
-    if (e >= 0) d = dw / (1.f + expf(-le)) / (1.f + expf(le));
+    if (!softmax) m = fminf(m, 0.f);
+    const float a = softmax || le <= 0.f ? expf(le - m) : 1.f, b = expf(-fabsf(le));
+    const float s = e < 0 ? 0.f : softmax ? a : a / (1.f + b);
+    const float sum = warp_sum(s), share = sum > 0.f ? s / sum : 0.f;
+    // 1 - sigmoid(l) = exp(-l) / (1 + exp(-l)) or 1 / (1 + exp(l)).
+    const float rest = softmax ? 1.f : (le > 0.f ? b : 1.f) / (1.f + b);
+    d = share * (dw - warp_sum(share * dw)) * rest;
+  } else if (softmax) {
+    const float share = e >= 0 ? expf(le - top) * inv : 0.f;
+    all = warp_sum(share * dw);
+    d = share * (dw - all);
   } else {
-    top = warp_max(top);
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      l[i] = l[i] > -INFINITY ? expf(l[i] - top) : 0.f;
-      sum += l[i];
-    }
-    sum = warp_sum(sum);
-    const float inv = sum > 0 ? 1.f / sum : 0.f;
-    if (e >= 0) d = dw * expf(le - top) * inv;
-    const float all = warp_sum(d);
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) g[i] = -l[i] * inv * all;
+    const float b = expf(-fabsf(le));
+    d = e >= 0 ? dw * b / ((1.f + b) * (1.f + b)) : 0.f;  // s (1 - s), the same for -l
   }
+  // Equal choices: the first of them writes the sum of all. Under the plain
+  // softmax each holds the row's own term, which counts once.
+  float own = 0.f;
+  if (softmax && !S.renormalise && e >= 0) own = -expf(le - top) * inv * all;
+  float total = 0.f;
+  bool first = true;
   for (int j = 0; j < k; ++j) {
     const int ej = __shfl_sync(kAll, e, j);
-    const float dj = __shfl_sync(kAll, d, j);
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (lane * EPL + i == ej) g[i] += dj;
+    const float dj = __shfl_sync(kAll, d - own, j);
+    total += ej == e ? dj : 0.f;
+    first &= !(ej == e && j < lane);
   }
+  for (int v = lane; softmax && v < words; v += 32) {
+    Pack<T, VB> o;
+    if (!S.renormalise) {
+      const Pack<T, VB> p = ld_pack<T, VB>(row + v * N);
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int x = lane * EPL + i;
-    if (x < E && real) dlogits[t * ldd + x] = narrow<T, float>(poison ? NAN : g[i]);
+      for (int i = 0; i < N; ++i) {
+        const float l = widen(p.v[i]);
+        o.v[i] = narrow<T, float>(poison ? NAN : l > -INFINITY ? -expf(l - top) * inv * all : 0.f);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) o.v[i] = narrow<T, float>(poison ? NAN : 0.f);
+    }
+    if (real) st_pack_stream<T, VB>(to + v * N, o);
   }
+  __syncwarp();
+  if (real && e >= 0 && first && !poison) to[e] = narrow<T, float>(own + total);
 }
 
 // Lanes of a group: the row's lanes shared out among the groups, a power of
@@ -736,12 +761,6 @@ int row_lanes(const spmvb_router_spec& s, int tokens, int sm_count) {
   int lanes = 8;
   while (lanes < 32 && (lanes * 8 < s.experts || lanes < s.k || lanes < s.groups)) lanes *= 2;
   return (s.groups & (s.groups - 1)) == 0 ? lanes : 32;
-}
-
-int slots_for(int experts) {
-  int slots = 1;
-  while (slots * 32 < experts) slots *= 2;
-  return slots;
 }
 
 template <typename F>
@@ -957,15 +976,18 @@ spmvb_status spmvb_router_route_grad(spmvb_router R, spmvb_dtype dtype, int32_t 
   for (const RowSet* r : {&logits, &dlogits, &idx, &dw}) SPMVB_TRY(check_rows(*r, dev));
   for (const RowSet* r : {&logits, &idx, &dw}) SPMVB_TRY(check_apart(dlogits, *r));
   if (tokens == 0) return SPMVB_OK;
-  return with_logits(dtype, slots_for(S.experts), [&](auto tv, auto epl) -> spmvb_status {
+  const int vb = access_bytes(es, {{d_logits, ld_logits}, {d_dlogits, ld_dlogits}}, S.experts);
+  const auto run = [&](auto tv) -> spmvb_status {
     using T = decltype(tv);
-    route_grad_rows<T, decltype(epl)::value><<<static_cast<int>(ceil_div(tokens, kRouteThreads / 32)), kRouteThreads, 0, s>>>(
+    const auto kernel = vb == 16 ? route_grad_rows<T, 16> : vb == 8 ? route_grad_rows<T, 8> : route_grad_rows<T, sizeof(T)>;
+    kernel<<<static_cast<int>(ceil_div(tokens, kRouteThreads / 32)), kRouteThreads, 0, s>>>(
         S, static_cast<const T*>(d_logits), ld_logits, tokens, d_indices, d_dweights, static_cast<T*>(d_dlogits),
         ld_dlogits, R->ctx->index_err());
     count_launch();
     SPMVB_TRY_CUDA(cudaGetLastError());
     return SPMVB_OK;
-  });
+  };
+  return dtype == SPMVB_F32 ? run(float{}) : dtype == SPMVB_F16 ? run(__half{}) : run(__nv_bfloat16{});
 }
 
 spmvb_status spmvb_router_dispatch(spmvb_router R, spmvb_dtype dtype, int32_t tokens, int32_t width,
