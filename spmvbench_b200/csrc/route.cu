@@ -633,18 +633,19 @@ __global__ void __launch_bounds__(kRouteThreads, EPL > 8 ? 2 : 4)
 //   sigmoid           scale * s_j * (1 - s_j) * dw_j
 //   softmax           scale * p_e * ([e chosen] dw_e - g) for every expert
 //
-// A warp a row. The row is written in words of VB bytes as if nothing were
+// L lanes a row (8 where they hold the choices). The row is written in words of VB bytes as if nothing were
 // chosen; lane j then writes the j-th choice's own value, with those of equal
 // choices added.
-template <typename T, int VB>
+template <typename T, int VB, int L>
 __global__ void __launch_bounds__(kRouteThreads)
     route_grad_rows(spmvb_router_spec S, const T* __restrict__ logits, int64_t ld, int tokens,
                     const int* __restrict__ indices, const float* __restrict__ dweights, T* __restrict__ dlogits,
                     int64_t ldd, int* __restrict__ err) {
   constexpr int N = VB / sizeof(T);
-  const int lane = threadIdx.x & 31, w0 = blockIdx.x * (kRouteThreads / 32) + (threadIdx.x >> 5);
-  const bool real = w0 < tokens;  // a warp past the last token repeats it and writes nothing
-  const int64_t t = real ? w0 : tokens - 1;
+  const int lane = threadIdx.x & (L - 1);
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kRouteThreads + threadIdx.x) / L;
+  const bool real = t0 < tokens;  // lanes past the last token repeat it and write nothing
+  const int64_t t = real ? t0 : tokens - 1;
   const int k = S.k, words = S.experts / N;
   const bool softmax = S.score == SPMVB_SOFTMAX;
   const T* row = logits + t * ld;
@@ -652,7 +653,7 @@ __global__ void __launch_bounds__(kRouteThreads)
   const int loaded = lane < k ? __ldg(indices + t * k + lane) : -1;
   // Zeros need not wait for the loads.
   if (!softmax && real)
-    for (int v = lane; v < words; v += 32) {
+    for (int v = lane; v < words; v += L) {
       Pack<T, VB> o;
 #pragma unroll
       for (int i = 0; i < N; ++i) o.v[i] = narrow<T, float>(0.f);
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(kRouteThreads)
   bool poison = false;
   if (softmax) {
     float sum = 0.f;
-    for (int v = lane; v < words; v += 32) {
+    for (int v = lane; v < words; v += L) {
       const Pack<T, VB> p = ld_pack<T, VB>(row + v * N);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -676,10 +677,10 @@ __global__ void __launch_bounds__(kRouteThreads)
         top = fmaxf(top, l);
       }
     }
-    poison = __any_sync(kAll, poison);
+    poison = row_any<L>(poison);
     if (!S.renormalise) {
-      top = warp_max(top);
-      for (int v = lane; v < words; v += 32) {
+      top = unordered(row_max<L>(ordered(top)));
+      for (int v = lane; v < words; v += L) {
         const Pack<T, VB> p = ld_pack<T, VB>(row + v * N);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -687,26 +688,26 @@ __global__ void __launch_bounds__(kRouteThreads)
           sum += l > -INFINITY ? expf(l - top) : 0.f;
         }
       }
-      sum = warp_sum(sum);
+      sum = row_sum<L>(sum);
       inv = sum > 0.f ? 1.f / sum : 0.f;
     }
   }
   if (S.renormalise) {
-    float m = warp_max(le);
+    float m = unordered(row_max<L>(ordered(le)));
     if (!softmax) m = fminf(m, 0.f);
     const float a = softmax || le <= 0.f ? expf(le - m) : 1.f, b = expf(-fabsf(le));
-    const float s = e < 0 ? 0.f : softmax ? a : a / (1.f + b);
-    const float sum = warp_sum(s), share = sum > 0.f ? s / sum : 0.f;
+    const float s = e < 0 ? 0.f : softmax ? a : __fdividef(a, 1.f + b);
+    const float sum = row_sum<L>(s), share = sum > 0.f ? __fdividef(s, sum) : 0.f;
     // 1 - sigmoid(l) = exp(-l) / (1 + exp(-l)) or 1 / (1 + exp(l)).
-    const float rest = softmax ? 1.f : (le > 0.f ? b : 1.f) / (1.f + b);
-    d = share * (dw - warp_sum(share * dw)) * rest;
+    const float rest = softmax ? 1.f : __fdividef(le > 0.f ? b : 1.f, 1.f + b);
+    d = share * (dw - row_sum<L>(share * dw)) * rest;
   } else if (softmax) {
     const float share = e >= 0 ? expf(le - top) * inv : 0.f;
-    all = warp_sum(share * dw);
+    all = row_sum<L>(share * dw);
     d = share * (dw - all);
   } else {
     const float b = expf(-fabsf(le));
-    d = e >= 0 ? dw * b / ((1.f + b) * (1.f + b)) : 0.f;  // s (1 - s), the same for -l
+    d = e >= 0 ? dw * __fdividef(b, (1.f + b) * (1.f + b)) : 0.f;  // s (1 - s), the same for -l
   }
   // Equal choices: the first of them writes the sum of all. Under the plain
   // softmax each holds the row's own term, which counts once.
@@ -714,13 +715,14 @@ __global__ void __launch_bounds__(kRouteThreads)
   if (softmax && !S.renormalise && e >= 0) own = -expf(le - top) * inv * all;
   float total = 0.f;
   bool first = true;
+#pragma unroll 4
   for (int j = 0; j < k; ++j) {
-    const int ej = __shfl_sync(kAll, e, j);
-    const float dj = __shfl_sync(kAll, d - own, j);
+    const int ej = __shfl_sync(kAll, e, j, L);
+    const float dj = __shfl_sync(kAll, d - own, j, L);
     total += ej == e ? dj : 0.f;
     first &= !(ej == e && j < lane);
   }
-  for (int v = lane; softmax && v < words; v += 32) {
+  for (int v = lane; softmax && v < words; v += L) {
     Pack<T, VB> o;
     if (!S.renormalise) {
       const Pack<T, VB> p = ld_pack<T, VB>(row + v * N);
@@ -979,8 +981,11 @@ spmvb_status spmvb_router_route_grad(spmvb_router R, spmvb_dtype dtype, int32_t 
   const int vb = access_bytes(es, {{d_logits, ld_logits}, {d_dlogits, ld_dlogits}}, S.experts);
   const auto run = [&](auto tv) -> spmvb_status {
     using T = decltype(tv);
-    const auto kernel = vb == 16 ? route_grad_rows<T, 16> : vb == 8 ? route_grad_rows<T, 8> : route_grad_rows<T, sizeof(T)>;
-    kernel<<<static_cast<int>(ceil_div(tokens, kRouteThreads / 32)), kRouteThreads, 0, s>>>(
+    const bool few = S.k <= 8;
+    const auto kernel = vb == 16  ? (few ? route_grad_rows<T, 16, 8> : route_grad_rows<T, 16, 32>)
+                        : vb == 8 ? (few ? route_grad_rows<T, 8, 8> : route_grad_rows<T, 8, 32>)
+                                  : (few ? route_grad_rows<T, sizeof(T), 8> : route_grad_rows<T, sizeof(T), 32>);
+    kernel<<<static_cast<int>(ceil_div(tokens, kRouteThreads / (few ? 8 : 32))), kRouteThreads, 0, s>>>(
         S, static_cast<const T*>(d_logits), ld_logits, tokens, d_indices, d_dweights, static_cast<T*>(d_dlogits),
         ld_dlogits, R->ctx->index_err());
     count_launch();
