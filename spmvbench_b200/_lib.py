@@ -196,4 +196,6 @@ def check(status: int, func: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args), name)
+    status = getattr(_lib or load(), name)(*args)
+    if status != OK:
+        check(status, name)

@@ -81,9 +81,36 @@ static AddrRangeFn addr_range_fn() {
   return fn;
 }
 
+// The same facts in one driver call for memory of `device`; false where the
+// answer is not that all is well.
+using PtrAttrFn = CUresult (*)(unsigned int, CUpointer_attribute*, void**, CUdeviceptr);
+static bool inside_device_memory(const void* p, size_t bytes, int device) {
+  static PtrAttrFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuPointerGetAttributes", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PtrAttrFn>(f);
+  }();
+  if (!fn) return false;
+  unsigned int type = 0, managed = 0;
+  int ordinal = -1;
+  CUdeviceptr base = 0;
+  size_t size = 0;
+  CUpointer_attribute what[] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL,
+                                CU_POINTER_ATTRIBUTE_RANGE_START_ADDR, CU_POINTER_ATTRIBUTE_RANGE_SIZE,
+                                CU_POINTER_ATTRIBUTE_IS_MANAGED};
+  void* to[] = {&type, &ordinal, &base, &size, &managed};
+  const auto at = reinterpret_cast<CUdeviceptr>(p);
+  return fn(5, what, to, at) == CUDA_SUCCESS && type == CU_MEMORYTYPE_DEVICE && !managed && ordinal == device &&
+         at >= base && bytes <= size && at - base <= size - bytes;
+}
+
 spmvb_status check_device_ptr(const void* p, size_t bytes, int device, const char* name) {
   if (bytes == 0) return SPMVB_OK;
   if (!p) return fail(SPMVB_ERR_INVALID_ARGUMENT, std::string(name) + " is null");
+  if (inside_device_memory(p, bytes, device)) return SPMVB_OK;
   cudaPointerAttributes at{};
   cudaError_t e = cudaPointerGetAttributes(&at, p);
   if (e != cudaSuccess) {

@@ -19,23 +19,26 @@ from . import _lib
 from ._lib import BF16, F16, F32, F64, call, load
 
 SCORES = {"softmax": 0, "sigmoid": 1}
-_CODES = None
+_CODES: dict = {}
+_raw_stream = None
 
 
-def _code(dtype):
-    """The library's code of a torch dtype, or None."""
-    global _CODES
-    if _CODES is None:
-        import torch
-        _CODES = {torch.float32: F32, torch.float64: F64, torch.float16: F16, torch.bfloat16: BF16}
-    return _CODES.get(dtype)
+def _torch_names() -> None:
+    """What the checks need of torch, looked up once (the package imports
+    without it)."""
+    global _raw_stream
+    import torch
+    _CODES.update({torch.float32: F32, torch.float64: F64, torch.float16: F16, torch.bfloat16: BF16,
+                   torch.int32: "int32"})
+    # The current stream's handle, without a Stream object around it.
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _stream(stream, device: int):
+def _stream(stream, device: int) -> int:
     if stream is None:
-        import torch
-        stream = torch.cuda.current_stream(device)
-    elif stream.device_index != device:
+        return _raw_stream(device)
+    if stream.device_index != device:
         raise ValueError(f"the stream belongs to cuda:{stream.device_index}, the handle to cuda:{device}")
     return stream.cuda_stream
 
@@ -47,27 +50,40 @@ def _on(t, device: int, what: str) -> None:
         raise ValueError(f"{what} is on cuda:{t.get_device()}, the handle on cuda:{device}")
 
 
-def _rows(t, rows, width: int, device: int, what: str, codes=(F32, F16, BF16)):
-    """Checks a rows x width tensor (rows None: any number) with unit column
-    stride; returns (dtype code, row stride)."""
-    _on(t, device, what)
-    code = _code(t.dtype)
+def _code(t, codes, device: int, what: str):
+    """The library's code of t's type, which must be one of `codes`; t must
+    be a CUDA tensor of `device`."""
+    if not _CODES:
+        _torch_names()
+    try:
+        code, at = _CODES.get(t.dtype), t.get_device()
+    except (AttributeError, RuntimeError):
+        code, at = None, -1
+    if at != device:
+        _on(t, device, what)
     if code not in codes:
         raise ValueError(f"{what} cannot be {t.dtype}")
+    return code
+
+
+def _rows(t, rows, width: int, device: int, what: str, codes=(F32, F16, BF16)):
+    """Checks a rows x width tensor (rows None: any number) with unit column
+    stride; returns (dtype code, row stride, address)."""
+    code = _code(t, codes, device, what)
     shape = t.shape
     if len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows):
         raise ValueError(f"{what} has shape {tuple(shape)}; ({'any' if rows is None else rows}, {width}) is needed")
     ld, unit = t.stride()
-    if (unit != 1 and width > 1) or (ld < width and shape[0] > 1):
-        raise ValueError(f"{what} must have rows of unit stride that do not overlap (strides {tuple(t.stride())})")
-    return code, max(ld, width)
+    if unit != 1 or ld < width:
+        if (unit != 1 and width > 1) or (ld < width and shape[0] > 1):
+            raise ValueError(f"{what} must have rows of unit stride that do not overlap (strides {t.stride()})")
+        ld = max(ld, width)
+    return code, ld, t.data_ptr()
 
 
-def _flat(t, dtype: str, count: int, device: int, what: str) -> int:
+def _flat(t, code, count: int, device: int, what: str) -> int:
     """Checks a contiguous tensor of `count` entries; returns its address."""
-    _on(t, device, what)
-    if str(t.dtype) != dtype:
-        raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
+    _code(t, (code,), device, what)
     if t.numel() != count:
         raise ValueError(f"{what} holds {t.numel()} entries; {count} are needed")
     if not t.is_contiguous():
@@ -75,7 +91,8 @@ def _flat(t, dtype: str, count: int, device: int, what: str) -> int:
     return t.data_ptr()
 
 
-I32, FLOAT32 = "torch.int32", "torch.float32"
+I32 = "int32"
+_ALL = (F32, F64, F16, BF16)
 
 
 class _Handle:
@@ -112,10 +129,10 @@ class Embedding(_Handle):
         zeros. tokens: int32, any shape, `count` entries; out: count x width."""
         dev, width = self.ctx.device, self.width
         count = tokens.numel()
-        code, ld = _rows(table, self.rows, width, dev, "table", (F32, F64, F16, BF16))
-        out_code, ldo = _rows(out, count, width, dev, "out", (code,))
+        code, ld, table_at = _rows(table, self.rows, width, dev, "table", _ALL)
+        _, ldo, out_at = _rows(out, count, width, dev, "out", (code,))
         call("spmvb_embedding_lookup", self.handle, code, count, _flat(tokens, I32, count, dev, "tokens"), scale,
-             table.data_ptr(), ld, out.data_ptr(), ldo, _stream(stream, dev))
+             table_at, ld, out_at, ldo, _stream(stream, dev))
 
     def lookup_grad(self, tokens, dout, dtable, scale: float = 1.0, accumulate: bool = False, stream=None) -> None:
         """dtable[r] = scale * sum of dout[t] over the tokens that name r, 0
@@ -123,10 +140,10 @@ class Embedding(_Handle):
         dout's type or is float32."""
         dev, width = self.ctx.device, self.width
         count = tokens.numel()
-        code, ldo = _rows(dout, count, width, dev, "dout", (F32, F64, F16, BF16))
-        grad_code, ld = _rows(dtable, self.rows, width, dev, "dtable", (code,) if code == F64 else (code, F32))
+        code, ldo, dout_at = _rows(dout, count, width, dev, "dout", _ALL)
+        grad_code, ld, dtable_at = _rows(dtable, self.rows, width, dev, "dtable", (code,) if code == F64 else (code, F32))
         call("spmvb_embedding_lookup_grad", self.handle, code, count, _flat(tokens, I32, count, dev, "tokens"), scale,
-             dout.data_ptr(), ldo, grad_code, dtable.data_ptr(), ld, int(accumulate), _stream(stream, dev))
+             dout_at, ldo, grad_code, dtable_at, ld, int(accumulate), _stream(stream, dev))
 
 
 class Router(_Handle):
@@ -156,10 +173,10 @@ class Router(_Handle):
         available (logit -inf or NaN). With offsets, order and position, also
         their plan (see plan)."""
         dev, k = self.ctx.device, self.k
-        code, ld = _rows(logits, None, self.experts, dev, "logits")
+        code, ld, logits_at = _rows(logits, None, self.experts, dev, "logits")
         tokens = logits.shape[0]
         n = tokens * k
-        b = None if bias is None else _flat(bias, FLOAT32, self.experts, dev, "bias")
+        b = None if bias is None else _flat(bias, F32, self.experts, dev, "bias")
         if offsets is None and order is None and position is None:
             plan = (None, None, None)
         elif offsets is None or order is None or position is None:
@@ -167,21 +184,21 @@ class Router(_Handle):
         else:
             plan = (_flat(offsets, I32, self.experts + 1, dev, "offsets"), _flat(order, I32, n, dev, "order"),
                     _flat(position, I32, n, dev, "position"))
-        call("spmvb_router_route", self.handle, code, tokens, logits.data_ptr(), ld, b,
-             _flat(indices, I32, n, dev, "indices"), _flat(weights, FLOAT32, n, dev, "weights"), *plan,
+        call("spmvb_router_route", self.handle, code, tokens, logits_at, ld, b,
+             _flat(indices, I32, n, dev, "indices"), _flat(weights, F32, n, dev, "weights"), *plan,
              _stream(stream, dev))
 
     def route_grad(self, logits, indices, dweights, dlogits, stream=None) -> None:
         """dlogits (all of it) from the weights' gradient, the choice in
         `indices` held fixed."""
         dev = self.ctx.device
-        code, ld = _rows(logits, None, self.experts, dev, "logits")
+        code, ld, logits_at = _rows(logits, None, self.experts, dev, "logits")
         tokens = logits.shape[0]
-        _, ldd = _rows(dlogits, tokens, self.experts, dev, "dlogits", (code,))
+        _, ldd, dlogits_at = _rows(dlogits, tokens, self.experts, dev, "dlogits", (code,))
         n = tokens * self.k
-        call("spmvb_router_route_grad", self.handle, code, tokens, logits.data_ptr(), ld,
-             _flat(indices, I32, n, dev, "indices"), _flat(dweights, FLOAT32, n, dev, "dweights"), dlogits.data_ptr(),
-             ldd, _stream(stream, dev))
+        call("spmvb_router_route_grad", self.handle, code, tokens, logits_at, ld,
+             _flat(indices, I32, n, dev, "indices"), _flat(dweights, F32, n, dev, "dweights"), dlogits_at, ldd,
+             _stream(stream, dev))
 
     def plan(self, indices, offsets, order, position, stream=None) -> None:
         """The choice by expert: expert e's rows are offsets[e] ..
@@ -198,46 +215,45 @@ class Router(_Handle):
 
     def _exchange(self, position, by_token, by_row, by_token_name: str, by_row_name: str):
         """Checks the two row sets of an exchange; returns (code, tokens,
-        width, position, stride by token, rows, stride by row)."""
+        width, position, by_token, its stride, rows, by_row, its stride)."""
         dev = self.ctx.device
         if len(getattr(by_token, "shape", ())) != 2:
             raise ValueError(f"{by_token_name} must be a matrix")
         tokens, width = by_token.shape
-        code, ld = _rows(by_token, tokens, width, dev, by_token_name)
-        _, ldr = _rows(by_row, None, width, dev, by_row_name, (code,))
-        return code, tokens, width, _flat(position, I32, tokens * self.k, dev, "position"), ld, by_row.shape[0], ldr
+        code, ld, at = _rows(by_token, tokens, width, dev, by_token_name)
+        _, ldr, row_at = _rows(by_row, None, width, dev, by_row_name, (code,))
+        return code, tokens, width, _flat(position, I32, tokens * self.k, dev, "position"), at, ld, by_row.shape[0], row_at, ldr
 
     def dispatch(self, position, X, out, stream=None) -> None:
         """out[position[t, j]] = X[t]; rows that no position names are left."""
-        code, tokens, width, pos, ld, rows, ldr = self._exchange(position, X, out, "X", "out")
-        call("spmvb_router_dispatch", self.handle, code, tokens, width, pos, X.data_ptr(), ld, rows, out.data_ptr(), ldr,
+        code, tokens, width, pos, at, ld, rows, row_at, ldr = self._exchange(position, X, out, "X", "out")
+        call("spmvb_router_dispatch", self.handle, code, tokens, width, pos, at, ld, rows, row_at, ldr,
              _stream(stream, self.ctx.device))
 
     def dispatch_grad(self, position, dout, dX, stream=None) -> None:
         """dX[t] = sum over j of dout[position[t, j]]."""
-        code, tokens, width, pos, ld, rows, ldr = self._exchange(position, dX, dout, "dX", "dout")
-        call("spmvb_router_dispatch_grad", self.handle, code, tokens, width, pos, rows, dout.data_ptr(), ldr,
-             dX.data_ptr(), ld, _stream(stream, self.ctx.device))
+        code, tokens, width, pos, at, ld, rows, row_at, ldr = self._exchange(position, dX, dout, "dX", "dout")
+        call("spmvb_router_dispatch_grad", self.handle, code, tokens, width, pos, rows, row_at, ldr, at, ld,
+             _stream(stream, self.ctx.device))
 
     def combine(self, position, weights, Y, out, stream=None) -> None:
         """out[t] = sum over j of weights[t, j] * Y[position[t, j]]."""
-        code, tokens, width, pos, ld, rows, ldr = self._exchange(position, out, Y, "out", "Y")
+        code, tokens, width, pos, at, ld, rows, row_at, ldr = self._exchange(position, out, Y, "out", "Y")
         dev = self.ctx.device
         call("spmvb_router_combine", self.handle, code, tokens, width, pos,
-             _flat(weights, FLOAT32, tokens * self.k, dev, "weights"), rows, Y.data_ptr(), ldr, out.data_ptr(), ld,
-             _stream(stream, dev))
+             _flat(weights, F32, tokens * self.k, dev, "weights"), rows, row_at, ldr, at, ld, _stream(stream, dev))
 
     def combine_grad(self, position, weights, Y, dout, dY, dweights, stream=None) -> None:
         """dY[position[t, j]] = weights[t, j] * dout[t] (rows that no position
         names are left; positions are distinct) and dweights[t, j] = the
         inner product of dout[t] and Y[position[t, j]]."""
-        code, tokens, width, pos, ld, rows, ldr = self._exchange(position, dout, Y, "dout", "Y")
+        code, tokens, width, pos, at, ld, rows, row_at, ldr = self._exchange(position, dout, Y, "dout", "Y")
         dev = self.ctx.device
         n = tokens * self.k
-        _, ldd = _rows(dY, rows, width, dev, "dY", (code,))
+        _, ldd, dY_at = _rows(dY, rows, width, dev, "dY", (code,))
         call("spmvb_router_combine_grad", self.handle, code, tokens, width, pos,
-             _flat(weights, FLOAT32, n, dev, "weights"), rows, Y.data_ptr(), ldr, dout.data_ptr(), ld, dY.data_ptr(),
-             ldd, _flat(dweights, FLOAT32, n, dev, "dweights"), _stream(stream, dev))
+             _flat(weights, F32, n, dev, "weights"), rows, row_at, ldr, at, ld, dY_at, ldd,
+             _flat(dweights, F32, n, dev, "dweights"), _stream(stream, dev))
 
 
 def router_spec(experts: int, k: int, score: str = "softmax", renormalise: bool = True, scale: float = 1.0,
@@ -262,25 +278,23 @@ class GradClip(_Handle):
 
     def __init__(self, ctx, tensors):
         tensors = list(tensors)
-        dev = ctx.device
+        dev, codes = ctx.device, []
         for i, t in enumerate(tensors):
-            _on(t, dev, f"tensor {i}")
-            if _code(t.dtype) is None:
-                raise ValueError(f"tensor {i} cannot be {t.dtype}")
+            codes.append(_code(t, _ALL, dev, f"tensor {i}"))
             if not t.is_contiguous():
                 raise ValueError(f"tensor {i} must be contiguous")
         n = len(tensors)
         self._tensors, self._places = tensors, [t.data_ptr() for t in tensors]
         h = C.c_void_p()
         call("spmvb_clip_create", ctx.handle, n, (C.c_void_p * n)(*self._places),
-             (C.c_int64 * n)(*[t.numel() for t in tensors]), (C.c_int * n)(*[_code(t.dtype) for t in tensors]),
+             (C.c_int64 * n)(*[t.numel() for t in tensors]), (C.c_int * n)(*codes),
              C.byref(h))
         self.handle, self.ctx = h, ctx
 
     def _check(self, norm) -> int:
         if [t.data_ptr() for t in self._tensors] != self._places:
             raise ValueError("a tensor's storage has been replaced: make a new GradClip")
-        return _flat(norm, FLOAT32, 1, self.ctx.device, "norm")
+        return _flat(norm, F32, 1, self.ctx.device, "norm")
 
     def norm(self, norm, stream=None) -> None:
         """The norm into `norm` (one float32 on the device)."""

@@ -73,8 +73,8 @@ def test_matrices_refuse_16_bit_types():
 
 def test_tensors_that_are_refused_before_the_c_call():
     t = torch.zeros(4, 8)
-    for call in (lambda: selection._rows(t, 4, 8, 0, "t"), lambda: selection._flat(t, "torch.float32", 32, 0, "t"),
-                 lambda: selection._rows(None, 4, 8, 0, "t"), lambda: selection._flat([1.0], "torch.float32", 1, 0, "t")):
+    for call in (lambda: selection._rows(t, 4, 8, 0, "t"), lambda: selection._flat(t, S.F32, 32, 0, "t"),
+                 lambda: selection._rows(None, 4, 8, 0, "t"), lambda: selection._flat([1.0], S.F32, 1, 0, "t")):
         with pytest.raises(ValueError, match="CUDA"):
             call()
 
@@ -96,14 +96,14 @@ class FakeCuda:
 def test_strides_shapes_devices_and_types_that_are_refused():
     rows = lambda t, *a, device=0, **k: selection._rows(FakeCuda(t, device), *a, 0, "t", **k)  # noqa: E731
     t = torch.zeros(4, 8)
-    assert rows(t, 4, 8) == (S.F32, 8) and rows(t[:, :5], 4, 5) == (S.F32, 8) and rows(t[::2], None, 8) == (S.F32, 16)
-    assert rows(t[:1].expand(1, 8), 1, 8) == (S.F32, 8) and rows(t[:, :1], 4, 1) == (S.F32, 8)
+    assert rows(t, 4, 8) == (S.F32, 8, t.data_ptr()) and rows(t[:, 1:5], 4, 4) == (S.F32, 8, t.data_ptr() + 4)
+    assert rows(t[::2], None, 8)[1] == 16 and rows(t[:1].expand(1, 8), 1, 8)[1] == 8 and rows(t[:, :1], 4, 1)[1] == 8
     for bad in (lambda: rows(t, 3, 8), lambda: rows(t, 4, 7), lambda: rows(t.t(), 8, 4), lambda: rows(t[:, ::2], 4, 4),
                 lambda: rows(t[0], 4, 8), lambda: rows(t[:1].expand(4, 8), 4, 8), lambda: rows(t.int(), 4, 8),
                 lambda: rows(t.double(), 4, 8), lambda: rows(t, 4, 8, device=1)):
         with pytest.raises(ValueError):
             bad()
-    flat = lambda t, n, device=0: selection._flat(FakeCuda(t, device), "torch.int32", n, 0, "t")  # noqa: E731
+    flat = lambda t, n, device=0: selection._flat(FakeCuda(t, device), selection.I32, n, 0, "t")  # noqa: E731
     i = torch.zeros(6, dtype=torch.int32)
     assert flat(i.view(2, 3), 6) == i.data_ptr()
     for bad in (lambda: flat(i, 5), lambda: flat(i.long(), 6), lambda: flat(i[::2], 3), lambda: flat(i, 6, device=1)):
