@@ -1,12 +1,13 @@
 // The expert plan: a stable counting sort of the choices by expert, and its
 // shares of the kernels that make it (route.cu, plan.cu).
 //
-// A tile is the choices of a few tokens: its counts per expert are made by the
-// routing kernel while it has the choices (or by plan_counts). A block is up to
-// kPlanEntries choices in whole tiles: plan_scatter adds up the counts of all
-// tiles, before its block and in total, ranks its choices among the equal ones
-// before them and writes them to their places. The ranks follow the entries'
-// order, so the plan is stable and does not depend on timing.
+// A block is up to kPlanEntries choices of whole tokens, and has a count for
+// each expert: added up by the routing kernel, tile by tile, while it has the
+// choices (integer atomics: the sums do not depend on their order), or made by
+// plan_counts. plan_scatter adds up the counts of all blocks, before its own and
+// in total, ranks its choices among the equal ones before them and writes them
+// to their places. The ranks follow the entries' order, so the plan is stable
+// and does not depend on timing.
 #pragma once
 
 #include "select.cuh"
@@ -22,18 +23,19 @@ constexpr int kPlanMaxExperts = 1024;
 // Tokens of a tile, tiles of a block.
 inline int plan_tile_tokens(int k) { return std::min(32, 512 / k); }
 inline int plan_block_tiles(int k) { return kPlanEntries / (plan_tile_tokens(k) * k); }
-// Row length of the tiles' counts: whole 16-byte words of 16-bit counts.
-inline int plan_stride(int experts) { return (experts + 7) / 8 * 8; }
+// Row length of the blocks' counts: whole 16-byte words.
+inline int plan_stride(int experts) { return (experts + 3) / 4 * 4; }
 
 struct PlanView {
   const int* indices;
   int64_t entries;
   int experts, stride;
   int tile_entries, block_tiles;
-  int tiles;
-  uint16_t* counts;  // tiles x stride
-  int* prefix;       // tiles x stride, the choices of an expert in the tiles before (plan_scan)
+  int blocks;
+  int* counts;       // blocks x stride; 0 between calls
+  int* prefix;       // blocks x stride, the choices of an expert in the blocks before (plan_scan)
   int* totals;       // stride
+  unsigned* ticket;  // 0 between calls
   int *offsets, *order, *position;
   int* err;
 };
@@ -177,14 +179,14 @@ __device__ __forceinline__ void plan_alone(Load&& load, int n, int experts, int*
 
 // ---- host ------------------------------------------------------------------------
 struct PlanSpace {
-  DevBuf counts, prefix, totals;
+  DevBuf counts, prefix, totals, ticket;
   spmvb_status alloc(int64_t tokens, int k, int experts);
 };
 // Fills in everything but the outputs.
 PlanView plan_view(const PlanSpace& space, const int* indices, int64_t tokens, int k, int experts, int* err);
-// Enqueues the plan; `counted`: the tiles' counts have been made.
+// Enqueues the plan; `counted`: the blocks' counts have been made.
 spmvb_status launch_plan(const PlanView& P, bool counted, cudaStream_t s);
 // One block makes the whole plan, without counts.
-inline bool plan_is_one_block(const PlanView& P) { return P.tiles <= P.block_tiles; }
+inline bool plan_is_one_block(const PlanView& P) { return P.blocks <= 1; }
 
 }  // namespace spmvb

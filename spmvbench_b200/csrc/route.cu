@@ -555,8 +555,8 @@ __device__ __forceinline__ bool route_row(const RouteShape& S, const T* __restri
 }
 
 // A block takes the tokens of a tile, 32 / L rows a warp at a time. With a plan
-// it also leaves the tile's counts of each expert, or, if the tile is all
-// there is, the plan itself.
+// it also adds the tile's counts of each expert to its plan block's, or, if
+// the tile is all there is, makes the plan itself.
 enum class PlanPart { None, Counts, Whole };
 
 template <typename T, int L, int EPL, bool Bias>
@@ -620,8 +620,9 @@ __global__ void __launch_bounds__(kRouteThreads, EPL > 8 ? 2 : 4)
   if (part == PlanPart::None) return;
   __syncthreads();
   if (part == PlanPart::Counts) {
-    for (int e = threadIdx.x; e < P.stride; e += kRouteThreads)
-      P.counts[static_cast<int64_t>(blockIdx.x) * P.stride + e] = static_cast<uint16_t>(counts[e]);
+    int* to = P.counts + static_cast<int64_t>(blockIdx.x / P.block_tiles) * P.stride;
+    for (int e = threadIdx.x; e < E; e += kRouteThreads)
+      if (counts[e] > 0) atomicAdd(to + e, counts[e]);
   } else {
     plan_alone<2>([&](int i) { return shared[i]; }, n * k, E, P.err, counts, counts + kPlanWarps * E, sh, P.offsets, P.order,
                   P.position);
