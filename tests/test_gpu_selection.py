@@ -132,6 +132,69 @@ def test_lookup_grad_runs_that_meet_chunk_edges(ctx, runs):
     assert torch.equal(dtable.double(), grad_rows(tokens, dout, 3 * len(runs))[0])
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("count,rows,hot", [
+    (256, 40, 0.0), (257, 40, 0.3), (2048, 3000, 0.1), (2049, 3000, 0.1), (9000, 2000, 0.5), (16384, 131072, 0.02),
+    (16384, 7, 1.0), (16385, 50000, 0.3), (70000, 300, 0.2), (140000, 600000, 0.0), (600, 9_000_000, 0.2), (30, 9_000_000, 0.0),
+    (3000, 1_000_000, 0.0)])
+def test_lookup_grad_of_every_way_to_sort(ctx, count, rows, hot, accumulate):
+    """Every number of tokens that is sorted in its own way, with a token that
+    is most of a block's; two calls in a row (the scratch is left as it was
+    found), integers: exact."""
+    g = gen(count + rows)
+    tokens = tokens_of(count, rows, g, empty=0.05)
+    tokens = torch.where(torch.rand(count, generator=g, device=DEV) < hot, rows - 1, tokens).int()
+    E = S.Embedding(ctx, rows, 8, max_tokens=count)
+    for turn in range(2):
+        dout = torch.randint(-16, 17, (count, 8), generator=g, device=DEV).float()
+        dtable = torch.randint(-4, 5, (rows, 8), generator=g, device=DEV).float()
+        want = grad_rows(tokens, dout, rows)[0] + (dtable.double() if accumulate else 0)
+        E.lookup_grad(tokens, dout, dtable, accumulate=accumulate)
+        assert torch.equal(dtable.double(), want), turn
+        tokens = tokens.flip(0).contiguous()
+    ctx.check()
+
+
+def test_rows_of_any_alignment(ctx):
+    """Widths, strides and offsets of every remainder of a 16-byte word, for
+    each operator that moves rows; nothing beside the rows is written."""
+    g = gen(21)
+    for dtype in (torch.bfloat16, torch.float32):
+        for width in (1, 2, 3, 5, 7, 8, 9, 15, 16, 17, 23, 31, 64, 65):
+            for pad, shift in ((0, 0), (1, 0), (0, 1), (3, 5), (8, 4), (7, 8)):
+                rows = 11
+                X, xb = strided(rows, width, dtype, pad, shift)
+                X.copy_(randn(rows, width, g=g))
+                tokens = torch.tensor([3, -1, 10, 0, 10], dtype=torch.int32, device=DEV)
+                out, ob = strided(5, width, dtype, (pad + 3) % 9, (shift + 1) % 9)
+                E = S.Embedding(ctx, rows, width, max_tokens=5)
+                E.lookup(tokens, X, out)
+                assert torch.equal(out, rows_at(X, tokens).to(dtype))
+                outside_untouched(ob, out)
+                grad, gb = strided(rows, width, dtype, pad, (shift + 3) % 9)
+                E.lookup_grad(tokens[:4], out[:4], grad)
+                assert torch.equal(grad, grad_rows(tokens[:4], out[:4], rows)[0].to(dtype))
+                outside_untouched(gb, grad)
+                R = S.Router(ctx, 4, 2, max_tokens=5)
+                position = torch.tensor([[0, 7], [2, -1], [9, 4], [-1, -1], [1, 3]], dtype=torch.int32, device=DEV)
+                xs, sb = strided(rows, width, dtype, (pad + 1) % 9, (shift + 2) % 9)
+                R.dispatch(position, out, xs)
+                for t, j in ((0, 0), (0, 1), (1, 0), (2, 0), (2, 1), (4, 0), (4, 1)):
+                    assert torch.equal(xs[position[t, j]], out[t])
+                outside_untouched(sb, xs)
+                back, bb = strided(5, width, dtype, pad, (shift + 5) % 9)
+                one = torch.ones(5, 2, device=DEV)
+                R.combine(position, one, xs, back)
+                assert torch.equal(back, rows_at(xs, position).sum(1).to(dtype))
+                outside_untouched(bb, back)
+                dY, yb = strided(rows, width, dtype, pad, (shift + 7) % 9)
+                dw = torch.empty(5, 2, device=DEV)
+                R.combine_grad(position, one, xs, out, dY, dw)
+                assert torch.equal(dY[7], out[0]) and torch.equal(dY[2], out[1])
+                outside_untouched(yb, dY)
+    ctx.check()
+
+
 def test_lookup_and_its_gradient_are_adjoint(ctx):
     """<lookup(X), G> = <X, lookup_grad(G)>: exact in integers."""
     g = gen(8)
@@ -267,6 +330,40 @@ def test_route_between_scores_that_fp32_does_not_tell_apart(ctx, score, bias):
     assert torch.equal(indices.cpu(), choose(l, b, 8, score))
 
 
+@pytest.mark.parametrize("experts,k,score,groups,kept,top", [
+    (256, 8, "sigmoid", 8, 4, 2), (256, 8, "softmax", 1, 1, 1), (60, 4, "softmax", 1, 1, 1), (64, 8, "sigmoid", 8, 3, 1),
+    (96, 32, "sigmoid", 32, 16, 2), (1020, 8, "sigmoid", 17, 5, 2)])
+@pytest.mark.parametrize("levels,bias", [(1, True), (3, True), (3, False), (40, True)])
+def test_route_of_equal_scores(ctx, experts, k, score, groups, kept, top, levels, bias):
+    """Logits of few values, as of a router that begins at zero: every choice
+    is among equals, and goes to the lowest index."""
+    tokens = 1500  # enough for rows to share a warp
+    g = gen(experts + levels)
+    logits = torch.randint(0, levels, (tokens, experts), generator=g, device=DEV).float() / 8
+    b = torch.randint(0, levels, (experts,), generator=g, device=DEV).float() / 16 if bias else None
+    R = S.Router(ctx, experts, k, max_tokens=tokens, score=score, groups=groups, groups_kept=kept, group_top=top)
+    indices = torch.empty(tokens, k, dtype=torch.int32, device=DEV)
+    weights = torch.empty(tokens, k, device=DEV)
+    R.route(logits, indices, weights, bias=b)
+    some = slice(0, 150)
+    assert torch.equal(indices[some].cpu(), choose(logits[some].cpu(), None if b is None else b.cpu(), k, score, groups, kept, top))
+
+
+def test_route_many_tokens_is_route_few_tokens(ctx):
+    """Rows that share a warp choose as rows that have one, ragged ends and
+    all; both with their plans."""
+    for experts, k, bias in ((64, 8, False), (100, 6, True), (16, 2, True), (128, 16, False)):
+        logits, b = route_case(1300, experts, bias, torch.float32, experts)
+        R = S.Router(ctx, experts, k, max_tokens=1300, score="sigmoid")
+        whole = [torch.empty(1300, k, dtype=torch.int32, device=DEV), torch.empty(1300, k, device=DEV)]
+        part = [torch.empty_like(t) for t in whole]
+        R.route(logits, *whole, bias=b)
+        for a in range(0, 1300, 433):
+            R.route(logits[a:a + 433], part[0][a:a + 433], part[1][a:a + 433], bias=b)
+        assert torch.equal(whole[0], part[0])
+        check(whole[1], part[1].double(), weight_bound(logits, part[1].double(), experts), "weights")
+
+
 def test_route_rows_without_scores(ctx):
     """NaN and infinities: an unavailable expert under the sigmoid, a row
     without scores under the softmax."""
@@ -355,7 +452,8 @@ def test_route_grad_against_differences(ctx, score, renormalise):
 
 
 @pytest.mark.parametrize("experts,k,tokens,skew", [(1, 1, 1, 0), (8, 2, 3, 0), (256, 8, 700, 3), (1024, 4, 3000, 0),
-                                                   (511, 3, 1500, 1), (512, 3, 1500, 1), (4, 32, 2100, 0), (64, 8, 0, 0)])
+                                                   (511, 3, 1500, 1), (512, 3, 1500, 1), (4, 32, 2100, 0), (64, 8, 0, 0),
+                                                   (100, 8, 33000, 2), (257, 4, 70000, 0), (1024, 1, 5000, 1)])
 def test_plan(ctx, experts, k, tokens, skew):
     """Any indices: absent, repeated in a row, all one expert's."""
     g = gen(experts + tokens)
@@ -366,10 +464,13 @@ def test_plan(ctx, experts, k, tokens, skew):
     offsets = torch.full((R.experts + 1,), 9, dtype=torch.int32, device=DEV)
     order = torch.full((tokens * k,), -9, dtype=torch.int32, device=DEV)
     position = torch.full((tokens, k), 9, dtype=torch.int32, device=DEV)
-    R.plan(idx, offsets, order, position)
-    o, by, at = plan_of(idx, R.experts)
-    assert offsets.tolist() == o and position.flatten().tolist() == at
-    assert order.tolist() == by + [-9] * (tokens * k - len(by))
+    for turn in range(2):  # the scratch is left as it was found
+        R.plan(idx, offsets, order, position)
+        o, by, at = plan_of(idx, R.experts)
+        assert offsets.tolist() == o and position.flatten().tolist() == at
+        assert order[:len(by)].tolist() == by and (order[len(by):] == -9).all()
+        idx = idx.flip(0).contiguous() if turn == 0 else idx
+        order.fill_(-9)
     ctx.check()
 
 
