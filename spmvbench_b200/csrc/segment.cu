@@ -21,8 +21,8 @@
 // Gradient. dtable[r] = scale * sum of dout[t] over the tokens that name r:
 // in that order the tokens of one row are neighbours (a run). A block takes
 // chunks of 16 or 4 tokens and a range of columns and adds each run in
-// registers. A run no longer than a chunk belongs to the chunk where it begins,
-// whole. Of a longer one every chunk that holds some leaves its part in scratch (slot 0: the run came
+// registers. A run of up to 16 belongs to the chunk where it begins, whole. Of
+// a longer one every chunk that holds some leaves its part in scratch (slot 0: the run came
 // in from the chunk before, slot 1: it begins here and goes on); the last of
 // its blocks to arrive adds the parts in chunk order. A frequent token is so spread over
 // many blocks, in a fixed order of summation. Where the gradient is not added
@@ -540,16 +540,19 @@ __device__ __forceinline__ int run_reach(const uint32_t* keys, int count, uint32
 
 // Tokens of a chunk: few where they would not fill the GPU.
 constexpr int kChunk = 16, kSmallChunk = 4;
+// A longer run is added in parts.
+constexpr int kLongRun = 16;
 // Packs of a thread, `across` packs apart: 16 bytes in all, 4 packs at most.
 constexpr int packs_of(int bytes) { return bytes >= 16 ? 1 : 16 / bytes > 4 ? 4 : 16 / bytes; }
 
-template <typename T, typename G, int N, int Chunk, bool Self, bool Add>
+// Wide: a block's threads lie along one row.
+template <typename T, typename G, int N, int Chunk, bool Self, bool Add, bool Wide>
 __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * sizeof(G) > 16) ? 2 : N * sizeof(T) < 16 ? 3 : 4)
     grad_rows(GradView A, const T* __restrict__ dout, typename AccOf<T>::type scale, G* __restrict__ dtable) {
   using Acc = typename AccOf<T>::type;
   constexpr int VB = N * sizeof(T), M = packs_of(VB);
   constexpr int Batch = 4;  // rows loaded before the first is added
-  constexpr int Span = 3 * Chunk;
+  constexpr int Span = Chunk + 2 * kLongRun;
   constexpr int MaxDown = kGradThreads / kMinAcross;
   __shared__ __align__(16) uint32_t pairs[Self ? kSelfTokens : 4];
   __shared__ uint32_t self_keys[Self ? kSelfTokens : 1];
@@ -587,19 +590,19 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * si
     vals = self_vals;
   }
 
-  // A chunk's keys and tokens, with the chunk before and the one after it.
-  const int down = kGradThreads / A.across;
-  const int x = threadIdx.x % A.across, y = threadIdx.x / A.across;
+  // A chunk's keys and tokens, with kLongRun before and after it.
+  const int down = Wide ? 1 : kGradThreads / A.across;
+  const int x = Wide ? threadIdx.x : threadIdx.x % A.across, y = Wide ? 0 : threadIdx.x / A.across;
   for (int i = threadIdx.x; i < down * Span; i += kGradThreads) {
-    const int64_t at = (static_cast<int64_t>(block_x) * down + i / Span - 1) * Chunk + i % Span;
+    const int64_t at = (static_cast<int64_t>(block_x) * down + i / Span) * Chunk + i % Span - kLongRun;
     const bool in = at >= 0 && at < A.count;
     ck[i] = in ? keys[at] : 0xffffffffu;
     cv[i] = in ? vals[at] : 0;
   }
   __syncthreads();
   const int chunk = block_x * down + y, v0 = range * A.across * M + x;
-  const uint32_t* k = ck + y * Span + Chunk;
-  const int* t = cv + y * Span + Chunk;
+  const uint32_t* k = ck + y * Span + kLongRun;
+  const int* t = cv + y * Span + kLongRun;
   Acc* parts = static_cast<Acc*>(A.parts);
   const bool mine = chunk < A.chunks;
   // The runs that cross the chunk's edges: [first_begin, first_end) and
@@ -610,9 +613,9 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * si
   int begin = 0, end = Chunk;
   if (came_in) {
     int from = -1, to = 1;
-    while (from > -Chunk && k[from - 1] == k[0]) --from;
-    while (to < 2 * Chunk && k[to] == k[0]) ++to;
-    if (to - from <= Chunk) {  // short: the chunk before adds it
+    while (from > -kLongRun && k[from - 1] == k[0]) --from;
+    while (to < Chunk + kLongRun && k[to] == k[0]) ++to;
+    if (to - from <= kLongRun) {  // short: the chunk where it begins adds it
       came_in = false;
       begin = to;
     }
@@ -620,58 +623,65 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * si
   const bool through = came_in && k[0] == k[Chunk - 1];
   if (goes_on) {
     int from = Chunk - 1, to = Chunk + 1;
-    while (from > -Chunk && k[from - 1] == k[Chunk - 1]) --from;
-    while (to < 2 * Chunk && k[to] == k[Chunk - 1]) ++to;
-    if (to - from <= Chunk) {
+    while (from > -kLongRun && k[from - 1] == k[Chunk - 1]) --from;
+    while (to < Chunk + kLongRun && k[to] == k[Chunk - 1]) ++to;
+    if (to - from <= kLongRun) {
       goes_on = false;
       end = from < 0 ? Chunk : to;
     }
   }
   bool in_first = came_in;
-  int col[M];  // -1: past the row's end
-#pragma unroll
-  for (int m = 0; m < M; ++m) col[m] = v0 + m * A.across < A.packs ? (v0 + m * A.across) * N : -1;
+  const int across = Wide ? kGradThreads : A.across;
+  const int64_t c0 = static_cast<int64_t>(v0) * N;
+  const T* const dout_c = dout + c0;  // this thread's first column; the others lie m * across * N on
+  G* const dtable_c = dtable + c0;
   if (mine) {
     Acc sum[M][N] = {};
 #pragma unroll 1
     for (int b = begin; b < end; b += Batch) {
       Pack<T, VB> p[Batch][M];
       RowPack<G, N> old[Add ? Batch : 1][M];
+      uint32_t key[Batch];
+      bool done[Batch];  // the run ends with this token
 #pragma unroll
       for (int q = 0; q < Batch; ++q) {
         const int i = b + q;
-        if (i >= end || k[i] >= A.rows) continue;
-        const T* from = dout + t[i] * A.ldo;
+        key[q] = i < end ? k[i] : 0xffffffffu;
+        done[q] = i + 1 >= end || k[i + 1] != key[q];
+        if (key[q] >= A.rows) continue;
+        const T* from = dout_c + t[i] * A.ldo;
 #pragma unroll
         for (int m = 0; m < M; ++m)
-          if (col[m] >= 0) p[q][m] = ld_pack_stream<T, VB>(from + col[m]);
-        if (Add && (i + 1 == end || k[i + 1] != k[i])) {
-          const G* was = dtable + k[i] * A.ldt;
+          if (v0 + m * across < A.packs) p[q][m] = ld_pack_stream<T, VB>(from + m * across * N);
+        if (Add && done[q]) {
+          const G* was = dtable_c + key[q] * A.ldt;
 #pragma unroll
           for (int m = 0; m < M; ++m)
-            if (col[m] >= 0) old[Add ? q : 0][m].load(was + col[m]);
+            if (v0 + m * across < A.packs) old[Add ? q : 0][m].load(was + m * across * N);
         }
       }
 #pragma unroll
       for (int q = 0; q < Batch; ++q) {
-        const int i = b + q;
-        if (i >= end || k[i] >= A.rows) continue;
-        const uint32_t key = k[i];
+        if (key[q] >= A.rows) continue;
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
           for (int n = 0; n < N; ++n) sum[m][n] += widen(p[q][m].v[n]);
-        if (i + 1 < end && k[i + 1] == key) continue;
-        const bool part = in_first || (i == Chunk - 1 && goes_on);
-        Acc* to = parts + (static_cast<int64_t>(chunk) * 2 + (in_first ? 0 : 1)) * A.width;
-        G* row = dtable + key * A.ldt;
+        if (!done[q]) continue;
+        if (in_first || (b + q == Chunk - 1 && goes_on)) {
+          Acc* to = parts + (static_cast<int64_t>(chunk) * 2 + (in_first ? 0 : 1)) * A.width + c0;
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-          if (col[m] < 0) continue;
-          if (part) {
+          for (int m = 0; m < M; ++m)
+            if (v0 + m * across < A.packs) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) __stcg(to + col[m] + n, sum[m][n]);
-          } else {
+              for (int n = 0; n < N; ++n) __stcg(to + m * across * N + n, sum[m][n]);
+            }
+          __threadfence();
+        } else {
+          G* row = dtable_c + key[q] * A.ldt;
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            if (v0 + m * across >= A.packs) continue;
             constexpr int W = RowPack<G, N>::M;
             RowPack<G, N> o;
 #pragma unroll
@@ -680,10 +690,9 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * si
               if (Add) r += widen(old[Add ? q : 0][m].p[n / W].v[n % W]);
               o.p[n / W].v[n % W] = narrow<G, Acc>(r);
             }
-            o.store(row + col[m]);
+            o.store(row + m * across * N);
           }
         }
-        if (part) __threadfence();
         in_first = false;
 #pragma unroll
         for (int m = 0; m < M; ++m)
@@ -867,9 +876,15 @@ spmvb_status lookup_grad(spmvb_embedding E, const Sorted& sorted, EmptyRows Z, c
   const int64_t blocks = static_cast<int64_t>(A.chunk_blocks) * A.ranges + A.empty_blocks;
   if (blocks == 0) return SPMVB_OK;
   if (blocks > INT32_MAX) return fail(SPMVB_ERR_UNSUPPORTED, "too many tokens for one launch");
-  const auto kernel = self    ? (accumulate ? grad_rows<T, G, N, kSmallChunk, true, true> : grad_rows<T, G, N, kSmallChunk, true, false>)
-                      : small ? (accumulate ? grad_rows<T, G, N, kSmallChunk, false, true> : grad_rows<T, G, N, kSmallChunk, false, false>)
-                              : (accumulate ? grad_rows<T, G, N, kChunk, false, true> : grad_rows<T, G, N, kChunk, false, false>);
+  const auto pick = [&](auto add, auto wide) {
+    constexpr bool Add = decltype(add)::value, Wide = decltype(wide)::value;
+    return self    ? grad_rows<T, G, N, kSmallChunk, true, Add, Wide>
+           : small ? grad_rows<T, G, N, kSmallChunk, false, Add, Wide>
+                   : grad_rows<T, G, N, kChunk, false, Add, Wide>;
+  };
+  const bool wide = A.across == kGradThreads;
+  const auto kernel = accumulate ? (wide ? pick(std::true_type{}, std::true_type{}) : pick(std::true_type{}, std::false_type{}))
+                                 : (wide ? pick(std::false_type{}, std::true_type{}) : pick(std::false_type{}, std::false_type{}));
   kernel<<<static_cast<unsigned>(blocks), kGradThreads, 0, s>>>(A, static_cast<const T*>(dout.p), Acc(scale),
                                                                 static_cast<G*>(const_cast<void*>(dtable.p)));
   count_launch();
