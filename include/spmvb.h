@@ -517,7 +517,9 @@ spmvb_status spmvb_dist_pipeline_destroy(spmvb_dist_pipeline P);
  *    time, others in smaller pieces.
  *  - A negative index selects nothing: a zero row, or no contribution. An
  *    index past the end is left out in the same way and reported by
- *    spmvb_context_check.
+ *    spmvb_context_check. Positions (of the experts' rows) are distinct, as
+ *    spmvb_router_plan makes them; two entries with the same one would write
+ *    the same row.
  *  - Outputs may not overlap inputs.
  *  - Handles hold scratch memory: a handle is used by one stream at a time
  *    (a captured graph's replays count as uses). Nothing allocates after

@@ -250,6 +250,7 @@ spmvb_status spmvb_clip_create(spmvb_context ctx, int32_t count, void* const* h_
     SPMVB_TRY(C->sums.alloc(static_cast<size_t>(C->blocks) * 8));
     SPMVB_TRY(C->factor.alloc(8));
     SPMVB_TRY(C->ticket.alloc(4));
+    SPMVB_TRY(scratch_ready());
     C->spans = std::move(spans);
     *out = C.release();
     return SPMVB_OK;

@@ -610,11 +610,12 @@ __global__ void __launch_bounds__(kRouteThreads, EPL > 8 ? 2 : 4)
       const int64_t t = t0 + i;
       float weight;
       const int mine = route_exact<T, (EPL * L / 32 > 0 ? EPL * L / 32 : 1)>(wide, logits + t * ld, Bias ? bias : nullptr, weight);
-      if (ln >= k) continue;
-      indices[t * k + ln] = mine;
-      weights[t * k + ln] = weight;
-      if (part == PlanPart::Counts && mine >= 0) atomicAdd(&counts[mine], 1);
-      if (part == PlanPart::Whole) shared[i * k + ln] = mine;
+      if (ln < k) {
+        indices[t * k + ln] = mine;
+        weights[t * k + ln] = weight;
+        if (part == PlanPart::Counts && mine >= 0) atomicAdd(&counts[mine], 1);
+        if (part == PlanPart::Whole) shared[i * k + ln] = mine;
+      }
     }
   }
   if (part == PlanPart::None) return;
@@ -870,6 +871,7 @@ spmvb_status spmvb_router_create(spmvb_context ctx, const spmvb_router_spec* spe
     R->spec = *spec;
     R->max_tokens = max_tokens;
     SPMVB_TRY(R->plan.alloc(max_tokens, spec->k, spec->experts));
+    SPMVB_TRY(scratch_ready());
     *out = R.release();
     return SPMVB_OK;
   });
@@ -927,7 +929,7 @@ spmvb_status spmvb_router_route(spmvb_router R, spmvb_dtype dtype, int32_t token
   }
   const int tile = plan_tile_tokens(S.k);
   const PlanPart part = !plan ? PlanPart::None
-                        : tokens <= tile ? PlanPart::Whole
+                        : tokens > 0 && tokens <= tile ? PlanPart::Whole
                         : plan_is_one_block(P) ? PlanPart::None : PlanPart::Counts;
   if (tokens > 0) {
     const int L = row_lanes(S, tokens, R->ctx->sm_count);

@@ -358,21 +358,24 @@ __global__ void __launch_bounds__(kOrderThreads)
 #pragma unroll
     for (int q = 0; q < Rounds; ++q)
       key[q] = q < turns && i0 + q * 32 < count ? static_cast<uint32_t>(__ldg(src + i0 + q * 32)) : 0xffffffffu;
-    int own = 0, less = 0, all = 0;
+    unsigned mine = 0, less = 0;  // a bit a turn
+    int all = 0;
 #pragma unroll
     for (int q = 0; q < Rounds; ++q) {
-      if (q >= turns) break;
-      if (part == 0) key_of(static_cast<int>(key[q]), n, err);  // reports an index past the end
       const bool in = key[q] < n;
       const int hash = static_cast<int>(key[q] * 2654435761u >> hash_shift);
-      own += __popc(__ballot_sync(0xffffffffu, in && hash == part));
-      less += __popc(__ballot_sync(0xffffffffu, in && hash < part));
-      all += __popc(__ballot_sync(0xffffffffu, in));
+      mine |= static_cast<unsigned>(in && hash == part) << q;
+      less |= static_cast<unsigned>(in && hash < part) << q;
+      all += in;
     }
+    if (part == 0)
+      for (int q = 0; q < Rounds; ++q) key_of(static_cast<int>(key[q]), n, err);  // reports an index past the end
+    const int own_w = __reduce_add_sync(0xffffffffu, __popc(mine)), less_w = __reduce_add_sync(0xffffffffu, __popc(less)),
+              all_w = __reduce_add_sync(0xffffffffu, all);
     if (lane == 0) {
-      found[0][w] = own;
-      found[1][w] = less;
-      found[2][w] = all;
+      found[0][w] = own_w;
+      found[1][w] = less_w;
+      found[2][w] = all_w;
     }
     __syncthreads();
     int incl = found[0][lane], offset = found[1][lane];
@@ -390,7 +393,7 @@ __global__ void __launch_bounds__(kOrderThreads)
 #pragma unroll
     for (int q = 0; q < Rounds; ++q) {
       if (q >= turns) break;
-      const bool in = key[q] < n && static_cast<int>(key[q] * 2654435761u >> hash_shift) == part;
+      const bool in = mine >> q & 1u;
       const unsigned vote = __ballot_sync(0xffffffffu, in);
       if (in) {
         name_row(named, key[q], n);
@@ -542,6 +545,7 @@ __device__ __forceinline__ int run_reach(const uint32_t* keys, int count, uint32
 constexpr int kChunk = 16, kSmallChunk = 4;
 // A longer run is added in parts.
 constexpr int kLongRun = 16;
+
 // Packs of a thread, `across` packs apart: 16 bytes in all, 4 packs at most.
 constexpr int packs_of(int bytes) { return bytes >= 16 ? 1 : 16 / bytes > 4 ? 4 : 16 / bytes; }
 
@@ -727,32 +731,53 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * si
     const int head = joined[y][slot][0], tail = joined[y][slot][1];
     if (head < 0) continue;
     const uint32_t key = slot == 0 ? k[0] : k[Chunk - 1];
-#pragma unroll 1
+    // Several parts' loads in flight: a frequent token's are the longest chain of
+    // the kernel.
+    constexpr int W = RowPack<G, N>::M;
+    constexpr int kPartsAhead = 4;
+    RowPack<G, N> o[M];
+    G* row = dtable_c + key * A.ldt;
+    Acc sum[M][N];
+    const Acc* part = parts + (static_cast<int64_t>(head) * 2 + 1) * A.width + c0;
+#pragma unroll
     for (int m = 0; m < M; ++m) {
-      const int64_t c = static_cast<int64_t>(v0 + m * A.across) * N;
-      if (c >= A.width) continue;
-      constexpr int W = RowPack<G, N>::M;
-      RowPack<G, N> o;
-      G* dst = dtable + key * A.ldt + c;
-      if (Add) o.load(dst);
-      Acc sum[N];
-      const Acc* part = parts + (static_cast<int64_t>(head) * 2 + 1) * A.width + c;
+      if (v0 + m * across >= A.packs) continue;
+      if (Add) o[m].load(row + m * across * N);
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum[i] = __ldcg(part + i);
-      part += A.width;  // slot 0 of the next chunk
-#pragma unroll 4
-      for (int q = head + 1; q <= tail; ++q) {
-        const Acc* from = part + static_cast<int64_t>(q - head - 1) * 2 * A.width;
+      for (int n = 0; n < N; ++n) sum[m][n] = __ldcg(part + m * across * N + n);
+    }
+    part += A.width;  // slot 0 of the next chunk
+    for (int q = head + 1; q <= tail; q += kPartsAhead) {
+      Acc next[kPartsAhead][M][N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] += __ldcg(from + i);
+      for (int u = 0; u < kPartsAhead; ++u)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+          if (q + u <= tail && v0 + m * across < A.packs) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+              next[u][m][n] = __ldcg(part + static_cast<int64_t>(u) * 2 * A.width + m * across * N + n);
+          }
+#pragma unroll
+      for (int u = 0; u < kPartsAhead; ++u)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+          if (q + u <= tail) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) sum[m][n] += next[u][m][n];
+          }
+      part += static_cast<int64_t>(kPartsAhead) * 2 * A.width;
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      if (v0 + m * across >= A.packs) continue;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        Acc r = sum[m][n] * scale;
+        if (Add) r += widen(o[m].p[n / W].v[n % W]);
+        o[m].p[n / W].v[n % W] = narrow<G, Acc>(r);
       }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        Acc r = sum[i] * scale;
-        if (Add) r += widen(o.p[i / W].v[i % W]);
-        o.p[i / W].v[i % W] = narrow<G, Acc>(r);
-      }
-      o.store(dst);
+      o[m].store(row + m * across * N);
     }
   }
 }
@@ -934,6 +959,7 @@ spmvb_status spmvb_embedding_create(spmvb_context ctx, int32_t rows, int32_t wid
     const size_t chunks = static_cast<size_t>(ceil_div(max_tokens, kSmallChunk));
     SPMVB_TRY(E->parts.alloc(chunks * 2 * width * 8));
     SPMVB_TRY(E->tickets.alloc(chunks * ceil_div(width, kGradThreads) * 4));
+    SPMVB_TRY(scratch_ready());
     *out = E.release();
     return SPMVB_OK;
   });

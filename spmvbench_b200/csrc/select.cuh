@@ -120,6 +120,13 @@ spmvb_status constructed(F&& f) {
   }
 }
 
+// New buffers are cleared on the legacy stream, which streams made without its
+// ordering do not wait for: a handle's first call may be on one of those.
+inline spmvb_status scratch_ready() {
+  SPMVB_TRY_CUDA(cudaStreamSynchronize(nullptr));
+  return SPMVB_OK;
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- row products (rows.cu) ------------------------------------------------------

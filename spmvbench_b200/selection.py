@@ -18,6 +18,7 @@ from operator import index as _as_int
 from . import _lib
 from ._lib import BF16, F16, F32, F64, call, load
 
+_MOST = 2 ** 31 - 1  # rows, entries: the C side counts in int32
 SCORES = {"softmax": 0, "sigmoid": 1}
 _CODES: dict = {}
 _raw_stream = None
@@ -71,7 +72,7 @@ def _rows(t, rows, width: int, device: int, what: str, codes=(F32, F16, BF16)):
     stride; returns (dtype code, row stride, address)."""
     code = _code(t, codes, device, what)
     shape = t.shape
-    if len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows):
+    if len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows) or shape[0] > _MOST:
         raise ValueError(f"{what} has shape {tuple(shape)}; ({'any' if rows is None else rows}, {width}) is needed")
     ld, unit = t.stride()
     if unit != 1 or ld < width:
@@ -84,7 +85,7 @@ def _rows(t, rows, width: int, device: int, what: str, codes=(F32, F16, BF16)):
 def _flat(t, code, count: int, device: int, what: str) -> int:
     """Checks a contiguous tensor of `count` entries; returns its address."""
     _code(t, (code,), device, what)
-    if t.numel() != count:
+    if t.numel() != count or count > _MOST:
         raise ValueError(f"{what} holds {t.numel()} entries; {count} are needed")
     if not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")

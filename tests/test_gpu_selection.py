@@ -364,6 +364,39 @@ def test_route_many_tokens_is_route_few_tokens(ctx):
         check(whole[1], part[1].double(), weight_bound(logits, part[1].double(), experts), "weights")
 
 
+def test_route_no_tokens(ctx):
+    R = S.Router(ctx, 12, 3, max_tokens=0)
+    none = dict(device=DEV, dtype=torch.int32)
+    offsets = torch.full((13,), 5, **none)
+    R.route(torch.empty(0, 12, device=DEV), torch.empty(0, 3, **none), torch.empty(0, 3, device=DEV), offsets=offsets,
+            order=torch.empty(0, **none), position=torch.empty(0, 3, **none))
+    assert not offsets.any()
+    R.route_grad(torch.empty(0, 12, device=DEV), torch.empty(0, 3, **none), torch.empty(0, 3, device=DEV),
+                 torch.empty(0, 12, device=DEV))
+
+
+def test_first_calls_on_a_stream_of_their_own(ctx):
+    """A handle's scratch is ready when create returns, also for a stream that
+    does not wait for the default one."""
+    g = gen(33)
+    tokens = tokens_of(9000, 700, g)
+    dout = torch.randint(-8, 9, (9000, 16), generator=g, device=DEV).float()
+    want = grad_rows(tokens, dout, 700)[0]
+    idx = torch.randint(0, 500, (9000, 4), generator=g, device=DEV, dtype=torch.int32)
+    o, by, at = plan_of(idx, 500)
+    side = torch.cuda.Stream()
+    dtable = torch.empty(700, 16, device=DEV)
+    plan = [torch.empty(n, dtype=torch.int32, device=DEV) for n in (501, 36000, 36000)]
+    torch.cuda.synchronize()
+    for turn in range(5):
+        E, R = S.Embedding(ctx, 700, 16, max_tokens=9000), S.Router(ctx, 500, 4, max_tokens=9000)
+        E.lookup_grad(tokens, dout, dtable, stream=side)
+        R.plan(idx, *plan, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(dtable.double(), want)
+        assert plan[0].tolist() == o and plan[1].tolist() == by and plan[2].tolist() == at
+
+
 def test_route_rows_without_scores(ctx):
     """NaN and infinities: an unavailable expert under the sigmoid, a row
     without scores under the softmax."""

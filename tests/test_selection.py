@@ -111,6 +111,23 @@ def test_strides_shapes_devices_and_types_that_are_refused():
             bad()
 
 
+def test_counts_past_int32_are_refused():
+    class Long(FakeCuda):
+        shape = (2 ** 31, 8)
+
+        def __init__(self):
+            super().__init__(torch.zeros(1, 8))
+            self.shape = (2 ** 31, 8)
+
+        def numel(self):
+            return 2 ** 31
+
+    with pytest.raises(ValueError):
+        selection._flat(Long(), S.F32, 2 ** 31, 0, "t")
+    with pytest.raises(ValueError):
+        selection._rows(Long(), None, 8, 0, "t")
+
+
 def test_plain_forms_by_hand():
     l = torch.tensor([[1.0, 3.0, 3.0, 0.0], [-math.inf, 2.0, -math.inf, -math.inf], [-math.inf] * 4])
     assert choose(l, None, 2, "softmax").tolist() == [[1, 2], [1, -1], [-1, -1]]
