@@ -572,7 +572,7 @@ spmvb_status launch_gather_sum(spmvb_dtype dtype, const int* idx, const float* w
       if (k > 1 && k <= kFew) {
         const int x = across(words, kWordsHeld, 1), y = kRowThreads / x;
         const auto few = w ? gather_sum_few<T, true> : gather_sum_few<T, false>;
-        SPMVB_TRY(w ? allow_shared<gather_sum_few<T, true>>() : allow_shared<gather_sum_few<T, false>>());
+        SPMVB_TRY((w ? allow_shared<gather_sum_few<T, true>>() : allow_shared<gather_sum_few<T, false>>()));
         few<<<static_cast<int>(ceil_div(count, y)), dim3(x, y), few_shared(k), s>>>(
             idx, w, count, k, static_cast<int>(X.rows), rows_at<const T>(X), X.ld, rows_at<T>(out), out.ld, words, err);
         return launched();
