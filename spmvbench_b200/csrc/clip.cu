@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kClipThreads, kClipBlocks / 148)
   if (!last) return;
   __threadfence();
   s = 0;
-  for (int i = threadIdx.x; i < gridDim.x; i += kClipThreads) s += __ldcg(sums + i);
+  for (int i = threadIdx.x; i < gridDim.x; i += kClipThreads) s += ld_written(sums + i);
   s = clip_block_sum(s);
   if (threadIdx.x == 0) {
     *ticket = 0u;

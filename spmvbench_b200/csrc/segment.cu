@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * si
       if (v0 + m * across >= A.packs) continue;
       if (Add) o[m].load(row + m * across * N);
 #pragma unroll
-      for (int n = 0; n < N; ++n) sum[m][n] = __ldcg(part + m * across * N + n);
+      for (int n = 0; n < N; ++n) sum[m][n] = ld_written(part + m * across * N + n);
     }
     part += A.width;  // slot 0 of the next chunk
     for (int q = head + 1; q <= tail; q += kPartsAhead) {
@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * si
           if (q + u <= tail && v0 + m * across < A.packs) {
 #pragma unroll
             for (int n = 0; n < N; ++n)
-              next[u][m][n] = __ldcg(part + static_cast<int64_t>(u) * 2 * A.width + m * across * N + n);
+              next[u][m][n] = ld_written(part + static_cast<int64_t>(u) * 2 * A.width + m * across * N + n);
           }
 #pragma unroll
       for (int u = 0; u < kPartsAhead; ++u)

@@ -120,6 +120,19 @@ spmvb_status constructed(F&& f) {
   }
 }
 
+// A load of what another block has written: not moved before the fence it
+// comes after, as the read-only loads (__ldg, __ldcg) may be.
+__device__ __forceinline__ double ld_written(const double* p) {
+  double r;
+  asm volatile("ld.global.cg.f64 %0, [%1];" : "=d"(r) : "l"(p) : "memory");
+  return r;
+}
+__device__ __forceinline__ float ld_written(const float* p) {
+  float r;
+  asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(r) : "l"(p) : "memory");
+  return r;
+}
+
 // New buffers are cleared on the legacy stream, which streams made without its
 // ordering do not wait for: a handle's first call may be on one of those.
 inline spmvb_status scratch_ready() {
