@@ -526,7 +526,8 @@ spmvb_status spmvb_dist_pipeline_destroy(spmvb_dist_pipeline P);
  *    create and nothing synchronizes, so every call can be captured.
  *  - Results do not depend on timing: sums have a fixed order. */
 typedef struct spmvb_embedding_st* spmvb_embedding;
-/* Scratch for the gradient of up to max_tokens rows of a rows x width table. */
+/* Scratch for the gradient of up to max_tokens rows of a rows x width table:
+ * about max_tokens * width bytes, and an eighth of a byte a row. */
 spmvb_status spmvb_embedding_create(spmvb_context ctx, int32_t rows,
                                     int32_t width, int32_t max_tokens,
                                     spmvb_embedding* out);

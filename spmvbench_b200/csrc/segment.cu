@@ -859,6 +859,7 @@ spmvb_status order_tokens_by_row(SortSpace& space, const int* idx, int count, in
 struct spmvb_embedding_st {
   spmvb_context ctx = nullptr;
   int device = 0, rows = 0, width = 0, max_tokens = 0;
+  int64_t chunks = 0;  // that parts and tickets are for
   spmvb::SortSpace sort;
   spmvb::DevBuf parts;    // 2 rows of sums (fp64 wide) per chunk
   spmvb::DevBuf tickets;  // one per chunk and column range, 0 between calls
@@ -890,6 +891,7 @@ spmvb_status lookup_grad(spmvb_embedding E, const Sorted& sorted, EmptyRows Z, c
   // Small chunks where large ones leave the SMs short of blocks.
   const bool small = self || ceil_div(ceil_div(count, kChunk), down) * A.ranges < E->ctx->sm_count;
   A.chunks = static_cast<int>(ceil_div(count, small ? kSmallChunk : kChunk));
+  if (A.chunks > E->chunks) return fail(SPMVB_ERR_UNSUPPORTED, "the handle's scratch does not hold the chunks");
   A.chunk_blocks = static_cast<int>(ceil_div(A.chunks, down));
   A.ldo = dout.ld;
   A.ldt = dtable.ld;
@@ -956,7 +958,13 @@ spmvb_status spmvb_embedding_create(spmvb_context ctx, int32_t rows, int32_t wid
     SPMVB_TRY(E->sort.alloc(max_tokens));
     SPMVB_TRY(E->named.alloc(static_cast<size_t>(ceil_div(rows, 32)) * 4));
     SPMVB_TRY_CUDA(cudaFuncSetAttribute(order_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize, kOrderShared));
-    const size_t chunks = static_cast<size_t>(ceil_div(max_tokens, kSmallChunk));
+    // Small chunks are taken up to the tokens that large ones would not make
+    // enough blocks of: with the fewest threads along a row (8 values each).
+    int across = kMinAcross;
+    while (across * 8 < width && across < kGradThreads) across *= 2;
+    const int64_t few = std::max<int64_t>(kSelfTokens, int64_t(ctx->sm_count) * kChunk * (kGradThreads / across));
+    E->chunks = std::max(ceil_div(max_tokens, kChunk), ceil_div(std::min<int64_t>(max_tokens, few), kSmallChunk));
+    const size_t chunks = static_cast<size_t>(E->chunks);
     SPMVB_TRY(E->parts.alloc(chunks * 2 * width * 8));
     SPMVB_TRY(E->tickets.alloc(chunks * ceil_div(width, kGradThreads) * 4));
     SPMVB_TRY(scratch_ready());
