@@ -517,7 +517,7 @@ struct GradView {
   int width, packs, across;   // columns, packs of them, threads along a row
   int64_t ldo, ldt;
   void* parts;
-  unsigned* tickets;  // chunks x ranges, all 0 between calls
+  unsigned* tickets;  // 3 a chunk and range, all 0 between calls
   EmptyRows empty;
   int* err;
 };
@@ -545,6 +545,14 @@ __device__ __forceinline__ int run_reach(const uint32_t* keys, int count, uint32
 constexpr int kChunk = 16, kSmallChunk = 4;
 // A longer run is added in parts.
 constexpr int kLongRun = 16;
+constexpr int kJoin = 16;  // chunks in a group, where the parts of a run are added by groups:
+constexpr int kJoinInGroups = 48;  // in runs that go on for so many chunks
+
+// Parts that a block adds: chunk * 2 + slot of the first and of the next, the
+// number after the first, and the groups besides this one that follow.
+struct Join {
+  int from, next, more, head, groups;
+};
 
 // Packs of a thread, `across` packs apart: 16 bytes in all, 4 packs at most.
 constexpr int packs_of(int bytes) { return bytes >= 16 ? 1 : 16 / bytes > 4 ? 4 : 16 / bytes; }
@@ -563,7 +571,7 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * si
   __shared__ int self_vals[Self ? kSelfTokens : 1];
   __shared__ uint32_t ck[MaxDown * Span];
   __shared__ int cv[MaxDown * Span];
-  __shared__ int joined[MaxDown][2][2];  // by slot: first and last chunk of a run whose parts are all there
+  __shared__ Join joined[MaxDown][2];  // by slot: what is to be added now
   const uint32_t* keys = A.keys;
   const int* vals = A.vals;
   // The blocks that write empty rows come last: their writes run at full rate
@@ -707,78 +715,124 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 8 || (Add && N * si
   }
   if (!__syncthreads_or(mine && (came_in || goes_on))) return;
   // Slot 0 is the run that came in, slot 1 one that begins here and goes on.
+  // The last block of a run to arrive adds its parts. In a run of
+  // kJoinInGroups chunks and more the last of each kJoin neighbours adds
+  // theirs, and the last of these the sums: a token that is all of 16,384 is a
+  // chain of 16 + 64 parts, not of 1,024.
+  unsigned* tickets = A.tickets + range;  // (chunk * 3 + which) * ranges on
   if (x < 2 && mine) {
-    const bool there = x == 0 ? came_in : goes_on && !through;
-    joined[y][x][0] = -1;
-    if (there) {
+    Join j;
+    j.from = -1;
+    if (x == 0 ? came_in : goes_on && !through) {
       const uint32_t key = x == 0 ? k[0] : k[Chunk - 1];
       const int head = x == 0 ? chunk - run_reach<Chunk>(keys, A.count, key, chunk, -1) : chunk;
       const int tail = x == 0 && !(through && goes_on) ? chunk : chunk + run_reach<Chunk>(keys, A.count, key, chunk, 1);
-      unsigned* ticket = A.tickets + static_cast<int64_t>(head) * A.ranges + range;
+      const bool grouped = tail - head >= kJoinInGroups;
+      const int first = grouped ? max(head, chunk / kJoin * kJoin) : head;
+      const int last = grouped ? min(tail, chunk / kJoin * kJoin + kJoin - 1) : tail;
+      unsigned* ticket = tickets + (static_cast<int64_t>(first) * 3 + (first == head)) * A.ranges;
       __threadfence();
-      if (atomicAdd(ticket, 1u) == static_cast<unsigned>(tail - head)) {
+      if (atomicAdd(ticket, 1u) == static_cast<unsigned>(last - first)) {
         *ticket = 0u;
         __threadfence();
-        joined[y][x][0] = head;
-        joined[y][x][1] = tail;
+        j.from = first * 2 + (first == head);
+        j.next = first * 2 + 2;
+        j.more = last - first;
+        j.head = head;
+        j.groups = grouped ? tail / kJoin - head / kJoin : 0;
       }
     }
+    joined[y][x] = j;
   }
   __syncthreads();
-  if (!mine) return;
+  // Several parts' loads in flight: a frequent token's are the longest chain of
+  // the kernel.
+  constexpr int kAhead = 4;
+  constexpr int W = RowPack<G, N>::M;
+  int step = 2;
 #pragma unroll 1
-  for (int slot = 0; slot < 2; ++slot) {
-    const int head = joined[y][slot][0], tail = joined[y][slot][1];
-    if (head < 0) continue;
-    const uint32_t key = slot == 0 ? k[0] : k[Chunk - 1];
-    // Several parts' loads in flight: a frequent token's are the longest chain of
-    // the kernel.
-    constexpr int W = RowPack<G, N>::M;
-    constexpr int kPartsAhead = 4;
-    RowPack<G, N> o[M];
-    G* row = dtable_c + key * A.ldt;
-    Acc sum[M][N];
-    const Acc* part = parts + (static_cast<int64_t>(head) * 2 + 1) * A.width + c0;
+  for (;;) {
+    bool on = false;  // a sum that waits for those of other groups
+#pragma unroll 1
+    for (int slot = 0; mine && slot < 2; ++slot) {
+      const Join j = joined[y][slot];
+      if (j.from < 0) continue;
+      G* row = dtable_c + (slot == 0 ? k[0] : k[Chunk - 1]) * A.ldt;
+      RowPack<G, N> o[M];
+      Acc sum[M][N];
+      Acc* from = parts + static_cast<int64_t>(j.from) * A.width + c0;
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      if (v0 + m * across >= A.packs) continue;
-      if (Add) o[m].load(row + m * across * N);
+      for (int m = 0; m < M; ++m)
+        if (v0 + m * across < A.packs) {
+          if (Add && j.groups == 0) o[m].load(row + m * across * N);
 #pragma unroll
-      for (int n = 0; n < N; ++n) sum[m][n] = ld_written(part + m * across * N + n);
-    }
-    part += A.width;  // slot 0 of the next chunk
-    for (int q = head + 1; q <= tail; q += kPartsAhead) {
-      Acc next[kPartsAhead][M][N];
+          for (int n = 0; n < N; ++n) sum[m][n] = ld_written(from + m * across * N + n);
+        }
+      const Acc* next = parts + static_cast<int64_t>(j.next) * A.width + c0;
+      for (int q = 0; q < j.more; q += kAhead, next += static_cast<int64_t>(kAhead * step) * A.width) {
+        Acc part[kAhead][M][N];
 #pragma unroll
-      for (int u = 0; u < kPartsAhead; ++u)
+        for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-        for (int m = 0; m < M; ++m)
-          if (q + u <= tail && v0 + m * across < A.packs) {
+          for (int m = 0; m < M; ++m)
+            if (q + u < j.more && v0 + m * across < A.packs) {
 #pragma unroll
-            for (int n = 0; n < N; ++n)
-              next[u][m][n] = ld_written(part + static_cast<int64_t>(u) * 2 * A.width + m * across * N + n);
-          }
+              for (int n = 0; n < N; ++n)
+                part[u][m][n] = ld_written(next + static_cast<int64_t>(u * step) * A.width + m * across * N + n);
+            }
 #pragma unroll
-      for (int u = 0; u < kPartsAhead; ++u)
+        for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-        for (int m = 0; m < M; ++m)
-          if (q + u <= tail) {
+          for (int m = 0; m < M; ++m)
+            if (q + u < j.more) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) sum[m][n] += next[u][m][n];
-          }
-      part += static_cast<int64_t>(kPartsAhead) * 2 * A.width;
-    }
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-      if (v0 + m * across >= A.packs) continue;
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        Acc r = sum[m][n] * scale;
-        if (Add) r += widen(o[m].p[n / W].v[n % W]);
-        o[m].p[n / W].v[n % W] = narrow<G, Acc>(r);
+              for (int n = 0; n < N; ++n) sum[m][n] += part[u][m][n];
+            }
       }
-      o[m].store(row + m * across * N);
+      if (j.groups > 0) {
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+          if (v0 + m * across < A.packs) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) __stcg(from + m * across * N + n, sum[m][n]);
+          }
+        __threadfence();
+        on = true;
+        continue;
+      }
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        if (v0 + m * across >= A.packs) continue;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          Acc r = sum[m][n] * scale;
+          if (Add) r += widen(o[m].p[n / W].v[n % W]);
+          o[m].p[n / W].v[n % W] = narrow<G, Acc>(r);
+        }
+        o[m].store(row + m * across * N);
+      }
     }
+    if (!__syncthreads_or(on)) return;
+    if (x < 2 && mine) {
+      Join j = joined[y][x];
+      const bool waits = j.from >= 0 && j.groups > 0;
+      j.from = -1;
+      if (waits) {
+        unsigned* ticket = tickets + (static_cast<int64_t>(j.head) * 3 + 2) * A.ranges;
+        __threadfence();
+        if (atomicAdd(ticket, 1u) == static_cast<unsigned>(j.groups)) {
+          *ticket = 0u;
+          __threadfence();
+          j.from = j.head * 2 + 1;
+          j.next = (j.head / kJoin + 1) * kJoin * 2;
+          j.more = j.groups;
+          j.groups = 0;
+        }
+      }
+      joined[y][x] = j;
+    }
+    step = 2 * kJoin;
+    __syncthreads();
   }
 }
 
@@ -862,7 +916,7 @@ struct spmvb_embedding_st {
   int64_t chunks = 0;  // that parts and tickets are for
   spmvb::SortSpace sort;
   spmvb::DevBuf parts;    // 2 rows of sums (fp64 wide) per chunk
-  spmvb::DevBuf tickets;  // one per chunk and column range, 0 between calls
+  spmvb::DevBuf tickets;  // 3 per chunk and column range, 0 between calls
   spmvb::DevBuf named;    // a bit per row, 0 between calls
 };
 
@@ -966,7 +1020,7 @@ spmvb_status spmvb_embedding_create(spmvb_context ctx, int32_t rows, int32_t wid
     E->chunks = std::max(ceil_div(max_tokens, kChunk), ceil_div(std::min<int64_t>(max_tokens, few), kSmallChunk));
     const size_t chunks = static_cast<size_t>(E->chunks);
     SPMVB_TRY(E->parts.alloc(chunks * 2 * width * 8));
-    SPMVB_TRY(E->tickets.alloc(chunks * ceil_div(width, kGradThreads) * 4));
+    SPMVB_TRY(E->tickets.alloc(chunks * 3 * ceil_div(width, kGradThreads) * 4));
     SPMVB_TRY(scratch_ready());
     *out = E.release();
     return SPMVB_OK;
