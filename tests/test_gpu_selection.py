@@ -155,6 +155,54 @@ def test_lookup_grad_of_every_way_to_sort(ctx, count, rows, hot, accumulate):
     ctx.check()
 
 
+@pytest.mark.parametrize("width", [8, 600, 4096])
+@pytest.mark.parametrize("runs", [
+    [188, 189, 190, 191, 192, 193, 194, 195, 196], [3, 752, 1, 767, 768, 769, 784], [1024, 16, 1023, 1025],
+    [12, 4096, 4, 2049, 7000], [1, 16383], [16384], [5, 20000, 64, 8192], [700] * 20])
+def test_lookup_grad_runs_over_many_chunks(ctx, runs, width):
+    """Rows that so many tokens name that their parts are added in steps: runs
+    of every place against those steps, beside each other. Integers, exact;
+    twice, with other tokens between."""
+    count, rows = sum(runs), 2 * len(runs) + 1
+    g = gen(count + width)
+    tokens = (2 * torch.repeat_interleave(torch.arange(len(runs)), torch.tensor(runs)) + 1).int().to(DEV)
+    E = S.Embedding(ctx, rows, width, max_tokens=count)
+    for turn in range(3):
+        use = tokens if turn != 1 else tokens[torch.randperm(count, generator=g, device=DEV)[: count // 2 + 1]]
+        dout = torch.randint(-8, 9, (use.numel(), width), generator=g, device=DEV).float()
+        dtable = torch.full((rows, width), 9.0, device=DEV)
+        E.lookup_grad(use, dout, dtable)
+        assert torch.equal(dtable.double(), grad_rows(use, dout, rows)[0]), turn
+    ctx.check()
+
+
+@pytest.mark.parametrize("rows", [3000, 100000])
+@pytest.mark.parametrize("share", [[0.5], [0.97], [0.2, 0.2, 0.2], [0.1, 0.05, 0.03, 0.02]])
+def test_lookup_grad_adds_in_token_order(ctx, share, rows):
+    """The order of a sum is the tokens' own: values whose fp32 sum depends on
+    it, as bits, for frequent rows in the middle, at the end and at the
+    beginning of the table."""
+    count, width = 9001, 4
+    g = gen(rows + len(share))
+    tokens = tokens_of(count, rows, g, empty=0.05)
+    u = torch.rand(count, generator=g, device=DEV)
+    for q, part in enumerate(share):
+        row = (rows // 2, rows - 1, 0, 7)[q]
+        tokens = torch.where((u >= 0) & (u < part), row, tokens).int()
+        u = u - part
+    dout = randn(count, width, g=g).float()
+    few = S.Embedding(ctx, rows, width, max_tokens=count)
+    dtable = torch.empty(rows, width, device=DEV)
+    few.lookup_grad(tokens, dout, dtable)
+    # The same tokens, sorted beforehand by a stable sort, with their rows:
+    # the same runs in the same places.
+    order = torch.argsort(torch.where(tokens < 0, rows, tokens), stable=True)
+    again = torch.empty_like(dtable)
+    few.lookup_grad(tokens[order].contiguous(), dout[order].contiguous(), again)
+    assert torch.equal(dtable, again)
+    ctx.check()
+
+
 def test_rows_of_any_alignment(ctx):
     """Widths, strides and offsets of every remainder of a 16-byte word, for
     each operator that moves rows; nothing beside the rows is written."""
