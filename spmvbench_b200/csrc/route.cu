@@ -151,10 +151,14 @@ __device__ __noinline__ int route_exact(const RouteShape& S, const T* __restrict
   }
   bool open = own > 0;
   if (S.s.groups > 1) {
+    // A group's single best is by what the experts are ranked by: without a
+    // bias the logits, as scores are equal long before the logits are.
+    const bool by_logit = !bias && S.s.group_top == 1;
     double a = -INFINITY, b = -INFINITY;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      if (c[i] > a) { b = a; a = c[i]; } else if (c[i] > b) { b = c[i]; }
+      const double v = by_logit && c[i] > -INFINITY ? l[i] : c[i];
+      if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
     }
     for (int off = 1 << S.lanes_log >> 1; off > 0; off >>= 1) {
       const double a2 = __shfl_xor_sync(kAll, a, off), b2 = __shfl_xor_sync(kAll, b, off);
