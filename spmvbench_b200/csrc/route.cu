@@ -222,6 +222,13 @@ __device__ __forceinline__ float reciprocal(float x) {
   return r;
 }
 
+// w / all, for 0 <= w <= all. Exactly 1 where one choice holds the whole sum: the
+// fast quotient of two equal values is a step below 1 for one value in five,
+// and a lone choice's gradient would not be 0.
+__device__ __forceinline__ float share_of(float w, float all) {
+  return w == all ? (all > 0.f ? 1.f : 0.f) : __fdividef(w, all);
+}
+
 // Maxima and sums over the L lanes of a row.
 template <int L>
 __device__ __forceinline__ uint32_t row_max(uint32_t v) {
@@ -549,7 +556,7 @@ __device__ __forceinline__ bool route_row(const RouteShape& S, const T* __restri
     }
     w = mine >= 0 ? w : 0.f;
     const float all = row_sum<L>(w);
-    w = all > 0.f ? __fdividef(w, all) : 0.f;
+    w = share_of(w, all);
   } else {
     w = softmax ? expf(ml - top) / sum : 1.f / (1.f + expf(-ml));
     w = mine >= 0 ? w : 0.f;
@@ -703,7 +710,7 @@ __global__ void __launch_bounds__(kRouteThreads)
     if (!softmax) m = fminf(m, 0.f);
     const float a = softmax || le <= 0.f ? expf(le - m) : 1.f, b = expf(-fabsf(le));
     const float s = e < 0 ? 0.f : softmax ? a : __fdividef(a, 1.f + b);
-    const float sum = row_sum<L>(s), share = sum > 0.f ? __fdividef(s, sum) : 0.f;
+    const float sum = row_sum<L>(s), share = share_of(s, sum);
     // 1 - sigmoid(l) = exp(-l) / (1 + exp(-l)) or 1 / (1 + exp(l)).
     const float rest = softmax ? 1.f : __fdividef(le > 0.f ? b : 1.f, 1.f + b);
     d = share * (dw - row_sum<L>(share * dw)) * rest;

@@ -66,3 +66,24 @@ def test_groups_of_saturated_scores(ctx, tokens, experts, k, groups, kept, score
     l = l.to(dtype)
     indices, _ = route(ctx, l, k, score=score, groups=groups, groups_kept=kept)
     assert torch.equal(indices, choose(l, None, k, score, groups, kept, 1))
+
+
+# ---- a lone choice ---------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("tokens", [150, 3000])
+def test_a_lone_choice_has_the_whole_weight(ctx, tokens, score, dtype):
+    """k = 1, renormalised: x / x is 1, so the weight is the scale and does not
+    depend on the logits; the same where masks leave one expert of many."""
+    g = torch.Generator().manual_seed(tokens)
+    l = (torch.randn(tokens, 64, generator=g) * 3).to(dtype)
+    lone = torch.full_like(l, -math.inf).scatter_(1, torch.randint(0, 64, (tokens, 1), generator=g), l[:, :1])
+    for logits, k in ((l, 1), (lone, 5)):
+        indices, weights = route(ctx, logits, k, score=score, scale=2.5)
+        assert (indices[:, 0] >= 0).all() and (indices[:, 1:] == -1).all()
+        assert (weights[:, 0] == 2.5).all() and not weights[:, 1:].any()
+        d = torch.full((tokens, 64), 7.0, device=DEV, dtype=dtype)
+        R = S.Router(ctx, 64, k, max_tokens=tokens, score=score, scale=2.5)
+        R.route_grad(logits.to(DEV), indices.to(DEV), torch.randn(tokens, k, generator=g).to(DEV), d)
+        assert not d.any()
