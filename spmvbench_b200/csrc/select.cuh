@@ -82,11 +82,17 @@ struct RowSet {
   int64_t rows, ld, width;
   size_t elem;
   const char* name;
+  // From the first row's begin to the last one's end (check_rows has seen that it fits).
   size_t bytes() const { return rows > 0 ? (static_cast<size_t>(rows - 1) * ld + width) * elem : 0; }
 };
 
 inline spmvb_status check_rows(const RowSet& s, int device) {
   if (s.ld < s.width) return fail(SPMVB_ERR_INVALID_ARGUMENT, std::string(s.name) + ": row stride below the row length");
+  // No sum or product of offsets within the rows may pass 63 bits: a length
+  // that wrapped would be found inside any allocation.
+  const int64_t most = INT64_MAX / static_cast<int64_t>(s.elem);
+  if (s.rows > 0 && (s.width > most || (s.rows > 1 && s.ld > (most - s.width) / (s.rows - 1))))
+    return fail(SPMVB_ERR_INVALID_ARGUMENT, std::string(s.name) + ": the rows' extent passes 63 bits");
   if (reinterpret_cast<uintptr_t>(s.p) % s.elem)
     return fail(SPMVB_ERR_INVALID_ARGUMENT, std::string(s.name) + " is not aligned to its elements");
   return check_device_ptr(s.p, s.bytes(), device, s.name);
@@ -97,8 +103,13 @@ inline spmvb_status check_rows(const RowSet& s, int device) {
 inline spmvb_status check_apart(const RowSet& out, const RowSet& in) {
   const auto a = reinterpret_cast<uintptr_t>(out.p), b = reinterpret_cast<uintptr_t>(in.p);
   if (!out.bytes() || !in.bytes() || a + out.bytes() <= b || b + in.bytes() <= a) return SPMVB_OK;
-  const int64_t row = out.ld * static_cast<int64_t>(out.elem);
-  if (row == in.ld * static_cast<int64_t>(in.elem) && row > 0) {
+  // The stride of a lone row may be anything.
+  const auto pitch = [](const RowSet& s) {
+    const int64_t e = static_cast<int64_t>(s.elem);
+    return s.ld <= INT64_MAX / e ? s.ld * e : 0;
+  };
+  const int64_t row = pitch(out);
+  if (row > 0 && row == pitch(in)) {
     int64_t off = (static_cast<int64_t>(b) - static_cast<int64_t>(a)) % row;
     if (off < 0) off += row;
     if (off >= out.width * static_cast<int64_t>(out.elem) && off + in.width * static_cast<int64_t>(in.elem) <= row)

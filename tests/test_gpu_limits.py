@@ -1,0 +1,68 @@
+"""Sizes and strides at the edge of what the row-selection operators and
+gradient clipping can index: refused before anything is launched, or right."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+import spmvbench_b200 as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def at(t):
+    return t.data_ptr()
+
+
+def refused(status, what):
+    message = S.load().spmvb_last_error().decode()
+    assert status == 1 and what in message, (status, message)
+
+
+@pytest.mark.parametrize("ld", [2 ** 58, 2 ** 60, 2 ** 62, 2 ** 63 - 1])
+def test_strides_whose_extent_wraps_are_refused(ctx, ld):
+    """17 rows 2^60 floats apart end 2^66 + 32 bytes on, which is 32 in 64 bits:
+    a length that any buffer has."""
+    lib = S.load()
+    rows, width = 17, 8
+    t = torch.zeros(rows, width, device=DEV)
+    u, v, x = torch.zeros_like(t), torch.zeros_like(t), torch.zeros_like(t)
+    i = torch.zeros(rows, dtype=torch.int32, device=DEV)
+    w = torch.zeros(rows, device=DEV)
+    torch.cuda.synchronize()
+    E = S.Embedding(ctx, rows, width, max_tokens=rows)
+    R = S.Router(ctx, width, 1, max_tokens=rows)
+    for a, b in ((ld, width), (width, ld)):
+        refused(lib.spmvb_embedding_lookup(E.handle, S.F32, rows, at(i), 1.0, at(t), a, at(u), b, None), "63 bits")
+        refused(lib.spmvb_embedding_lookup_grad(E.handle, S.F32, rows, at(i), 1.0, at(t), a, S.F32, at(u), b, 0, None), "63 bits")
+        refused(lib.spmvb_router_route_grad(R.handle, S.F32, rows, at(t), a, at(i), at(w), at(u), b, None), "63 bits")
+        refused(lib.spmvb_router_dispatch(R.handle, S.F32, rows, width, at(i), at(t), a, rows, at(u), b, None), "63 bits")
+        refused(lib.spmvb_router_dispatch_grad(R.handle, S.F32, rows, width, at(i), rows, at(t), a, at(u), b, None), "63 bits")
+        refused(lib.spmvb_router_combine(R.handle, S.F32, rows, width, at(i), at(w), rows, at(t), a, at(u), b, None), "63 bits")
+    refused(lib.spmvb_router_route(R.handle, S.F32, rows, at(t), ld, None, at(i), at(w), None, None, None, None), "63 bits")
+    for lds in ((ld, width, width), (width, ld, width), (width, width, ld)):
+        refused(lib.spmvb_router_combine_grad(R.handle, S.F32, rows, width, at(i), at(w), rows, at(t), lds[0], at(u), lds[1],
+                                              at(v), lds[2], at(x), None), "63 bits")
+    ctx.check()
+
+
+def test_a_lone_row_may_have_any_stride(ctx):
+    lib = S.load()
+    t, u = torch.arange(8.0, device=DEV).view(1, 8), torch.zeros(1, 8, device=DEV)
+    i = torch.zeros(1, dtype=torch.int32, device=DEV)
+    E = S.Embedding(ctx, 1, 8, max_tokens=1)
+    torch.cuda.synchronize()
+    for ld in (8, 2 ** 40, 2 ** 63 - 1):
+        u.zero_()
+        torch.cuda.synchronize()
+        assert lib.spmvb_embedding_lookup(E.handle, S.F32, 1, at(i), 1.0, at(t), ld, at(u), ld, None) == 0
+        ctx.check()
+        assert torch.equal(t, u)
+    # A row of columns beside it in the same buffer is not its own.
+    both = torch.arange(64.0, device=DEV).view(2, 32)
+    E = S.Embedding(ctx, 1, 16, max_tokens=2)
+    E.lookup(torch.zeros(2, dtype=torch.int32, device=DEV), both[:1, :16], both[:, 16:])
+    assert torch.equal(both[1, 16:], both[0, :16]) and torch.equal(both[0, 16:], both[0, :16])
