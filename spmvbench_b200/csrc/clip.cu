@@ -215,7 +215,11 @@ spmvb_status spmvb_clip_create(spmvb_context ctx, int32_t count, void* const* h_
     for (int32_t i = 0; i < count; ++i) {
       if (!any_float(h_dtypes[i])) return fail(SPMVB_ERR_INVALID_ARGUMENT, "tensor " + std::to_string(i) + ": bad dtype");
       if (h_sizes[i] < 0) return fail(SPMVB_ERR_INVALID_ARGUMENT, "tensor " + std::to_string(i) + ": negative size");
-      total += h_sizes[i] * static_cast<int64_t>(dtype_size(h_dtypes[i]));
+      const int64_t es = static_cast<int64_t>(dtype_size(h_dtypes[i]));
+      // No device holds that much, and past 63 bits the length would wrap.
+      if (h_sizes[i] > (INT64_MAX - total) / es)
+        return fail(SPMVB_ERR_INVALID_ARGUMENT, "tensor " + std::to_string(i) + ": the tensors' bytes pass 63 bits");
+      total += h_sizes[i] * es;
     }
     // Small pieces where large ones would leave SMs without any.
     int64_t piece = kMinPiece;

@@ -66,3 +66,15 @@ def test_a_lone_row_may_have_any_stride(ctx):
     E = S.Embedding(ctx, 1, 16, max_tokens=2)
     E.lookup(torch.zeros(2, dtype=torch.int32, device=DEV), both[:1, :16], both[:, 16:])
     assert torch.equal(both[1, 16:], both[0, :16]) and torch.equal(both[0, 16:], both[0, :16])
+
+
+@pytest.mark.parametrize("sizes,dtype", [([2 ** 61], S.F64), ([2 ** 62], S.F32), ([2 ** 63 - 1], S.BF16), ([2 ** 63 - 1], S.F64),
+                                         ([16, 2 ** 60 - 1], S.F64), ([2 ** 62 - 1] * 3, S.F16)])
+def test_clip_sizes_whose_bytes_wrap_are_refused(ctx, sizes, dtype):
+    """2^61 doubles are 2^64 bytes, 0 in 64 bits: a length that is in order for
+    any pointer."""
+    t = torch.zeros(16, device=DEV, dtype=torch.float64)
+    n, out = len(sizes), C.c_void_p()
+    refused(S.load().spmvb_clip_create(ctx.handle, n, (C.c_void_p * n)(*[at(t)] * n), (C.c_int64 * n)(*sizes),
+                                       (C.c_int * n)(*[dtype] * n), C.byref(out)), "63 bits")
+    assert not out.value
