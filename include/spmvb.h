@@ -162,7 +162,8 @@ spmvb_status spmvb_context_destroy(spmvb_context ctx);
  * this context gave up a bounded wait since the last check
  * (SPMVB_ERR_TIMEOUT; the word is then cleared), or whether a row-selection
  * operator met an index outside its range and left it out
- * (SPMVB_ERR_INVALID_ARGUMENT; likewise). The host-buffer entry
+ * (SPMVB_ERR_INVALID_ARGUMENT; likewise). One of the two a call: where both
+ * happened, the second call reports the other. The host-buffer entry
  * points perform the first check on their own stream before returning. */
 spmvb_status spmvb_context_check(spmvb_context ctx);
 /* Launches a kernel whose bounded wait can never be satisfied (an mbarrier

@@ -248,11 +248,16 @@ spmvb_status spmvb_context_check(spmvb_context ctx) {
   SPMVB_TRY_CUDA(cudaDeviceSynchronize());
   int code[2] = {0, 0};
   SPMVB_TRY_CUDA(cudaMemcpy(code, ctx->err.get(), sizeof(code), cudaMemcpyDeviceToHost));
-  if (code[0] != 0 || code[1] != 0) SPMVB_TRY_CUDA(cudaMemset(ctx->err.get(), 0, sizeof(code)));
-  if (code[0] != 0)
+  // Only the word that is reported is cleared: the other one waits for the
+  // next check.
+  if (code[0] != 0) {
+    SPMVB_TRY_CUDA(cudaMemset(ctx->err.get(), 0, sizeof(int)));
     return fail(SPMVB_ERR_TIMEOUT, "a kernel's bounded wait gave up (device error code " + std::to_string(code[0]) + ")");
-  if (code[1] != 0)
+  }
+  if (code[1] != 0) {
+    SPMVB_TRY_CUDA(cudaMemset(ctx->index_err(), 0, sizeof(int)));
     return fail(SPMVB_ERR_INVALID_ARGUMENT, "a row-selection operator met an index out of range and left it out");
+  }
   return SPMVB_OK;
 }
 

@@ -78,3 +78,16 @@ def test_clip_sizes_whose_bytes_wrap_are_refused(ctx, sizes, dtype):
     refused(S.load().spmvb_clip_create(ctx.handle, n, (C.c_void_p * n)(*[at(t)] * n), (C.c_int64 * n)(*sizes),
                                        (C.c_int * n)(*[dtype] * n), C.byref(out)), "63 bits")
     assert not out.value
+
+
+def test_a_timeout_does_not_swallow_the_report_of_an_index(ctx):
+    """A wait that gave up and an index past the end, before the same check:
+    both are reported, one after the other."""
+    E = S.Embedding(ctx, 4, 8, max_tokens=1)
+    out = torch.zeros(1, 8, device=DEV)
+    E.lookup(torch.full((1,), 9, dtype=torch.int32, device=DEV), torch.ones(4, 8, device=DEV), out)
+    assert S.load().spmvb_selftest_wait_timeout(ctx.handle) == 7
+    with pytest.raises(S.SpmvbError) as e:
+        ctx.check()
+    assert e.value.status == 1 and "out of range" in str(e.value)
+    ctx.check()
