@@ -645,9 +645,12 @@ spmvb_status spmvb_router_combine_grad(spmvb_router R, spmvb_dtype dtype,
 /* The 2-norm over many tensors at once, and their scaling by
  * min(1, max_norm / (norm + eps)) in place. The handle holds the tensors'
  * addresses (dense, `sizes` elements of `dtypes`; no two may overlap), which
- * must stay valid while it is used. Squares are summed in fp64. A norm that
- * is not finite carries on as the formula has it (NaN makes every gradient
- * NaN). No reference counterpart. */
+ * must stay valid while it is used. Squares are summed in fp64, those of
+ * doubles past 2^480 or below 2^-480 apart: finite values have a finite norm
+ * wherever fp64 holds it. The norm is handed out in fp32 (inf past its range);
+ * the factor is made from the fp64 one and multiplies in fp64 where fp32 does
+ * not hold it. A norm that is not finite carries on as the formula has it
+ * (NaN makes every gradient NaN). No reference counterpart. */
 typedef struct spmvb_clip_st* spmvb_clip;
 spmvb_status spmvb_clip_create(spmvb_context ctx, int32_t count,
                                void* const* h_tensors, const int64_t* h_sizes,

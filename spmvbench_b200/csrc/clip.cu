@@ -5,7 +5,9 @@
 // pieces in fp64; the last block to finish adds the blocks' sums in their order
 // and forms the factor. scale_pieces multiplies, from the last piece to the
 // first, so that it finds in the L2 what was read last, and leaves the tensors
-// alone where the factor is 1. HBM bounds both: the data is read twice and
+// alone where the factor is 1. Squares of doubles past 2^480 or below 2^-480 are
+// summed apart, scaled by a power of two: the norm of finite values is finite
+// where fp64 holds it. HBM bounds both: the data is read twice and
 // written once (no cache holds it in between). fp64 costs the bf16 sum nothing
 // yet: its conversions take 0.7 of the reading time.
 #include <cmath>
@@ -57,8 +59,35 @@ __device__ __forceinline__ Pack<T, 16> as_pack(const uint4& v) {
   return p;
 }
 
+// Sums of squares: of doubles past 2^480 in units of 2^1200, of those below
+// 2^-480 in units of 2^-1200, and of all other values. 2^40 squares of none of
+// the three leave fp64, and neither do those of any fp32 value.
+struct Squares {
+  double mid = 0, big = 0, small = 0;
+};
+constexpr double kBig = 0x1p480, kSmall = 0x1p-480, kUp = 0x1p600, kDown = 0x1p-600;
+
+// Adds x * x: to s where it is neither big nor small, which its exponent alone
+// tells (zeros are small; NaN goes to s).
+__device__ __forceinline__ void add_square(double x, double& s, Squares& far) {
+  constexpr unsigned Least = (1023u - 480u) << 20, Most = (1023u + 480u) << 20;
+  if ((static_cast<unsigned>(__double2hiint(x)) & 0x7fffffffu) - Least < Most - Least) {
+    s = fma(x, x, s);
+  } else if (fabs(x) >= kBig) {
+    far.big = fma(x * kDown, x * kDown, far.big);
+  } else if (fabs(x) < kSmall) {
+    far.small = fma(x * kUp, x * kUp, far.small);
+  } else {
+    s += x;
+  }
+}
+__device__ __forceinline__ void add_square(float x, double& s, Squares&) {
+  const double a = static_cast<double>(x);
+  s = fma(a, a, s);
+}
+
 template <typename T>
-__device__ __forceinline__ double piece_squares(const Piece& c) {
+__device__ __forceinline__ void piece_squares(const Piece& c, Squares& sum) {
   double s0 = 0, s1 = 0;
   each_word<T>(
       c,
@@ -66,16 +95,12 @@ __device__ __forceinline__ double piece_squares(const Piece& c) {
         const Pack<T, 16> x = as_pack<T>(v);
 #pragma unroll
         for (int i = 0; i < Pack<T, 16>::N; i += 2) {
-          const double a = static_cast<double>(widen(x.v[i])), b = static_cast<double>(widen(x.v[i + 1]));
-          s0 = fma(a, a, s0);
-          s1 = fma(b, b, s1);
+          add_square(widen(x.v[i]), s0, sum);
+          add_square(widen(x.v[i + 1]), s1, sum);
         }
       },
-      [&](const T* p) {
-        const double a = static_cast<double>(widen(*p));
-        s0 = fma(a, a, s0);
-      });
-  return s0 + s1;
+      [&](const T* p) { add_square(widen(*p), s0, sum); });
+  sum.mid += s0 + s1;
 }
 
 // Sum over the block, valid in thread 0.
@@ -92,6 +117,14 @@ __device__ __forceinline__ double clip_block_sum(double v) {
   return v;
 }
 
+__device__ __forceinline__ void clip_block_sums(Squares& s, bool doubles) {
+  s.mid = clip_block_sum(s.mid);
+  if (doubles && __syncthreads_or(s.big != 0 || s.small != 0)) {
+    s.big = clip_block_sum(s.big);
+    s.small = clip_block_sum(s.small);
+  }
+}
+
 // Calls f(T{}) for the type of a piece; Only: that of all tensors, or -1.
 template <int Only, typename F>
 __device__ __forceinline__ void with_piece(const Piece& c, F&& f) {
@@ -102,60 +135,117 @@ __device__ __forceinline__ void with_piece(const Piece& c, F&& f) {
   else f(__nv_bfloat16{});
 }
 
-// `ticket` is 0 between calls.
+// sums: mid of every block, then, where there are doubles, big and small.
+// factor: what values are multiplied by and, where there are doubles, a power of
+// two to multiply them by before. `ticket` is 0 between calls.
 template <int Only>
 __global__ void __launch_bounds__(kClipThreads, kClipBlocks / 148)
     sum_squares(const Piece* __restrict__ pieces, int count, double* __restrict__ sums, unsigned* __restrict__ ticket,
                 double max_norm, double eps, float* __restrict__ norm, double* __restrict__ factor) {
+  constexpr bool Doubles = Only < 0 || Only == SPMVB_F64;
   __shared__ bool last;
-  double s = 0;
+  Squares s;
   for (int c = blockIdx.x; c < count; c += gridDim.x) {
     const Piece q = pieces[c];
-    with_piece<Only>(q, [&](auto tv) { s += piece_squares<decltype(tv)>(q); });
+    with_piece<Only>(q, [&](auto tv) { piece_squares<decltype(tv)>(q, s); });
   }
-  s = clip_block_sum(s);
+  clip_block_sums(s, Doubles);
   if (threadIdx.x == 0) {
-    __stcg(sums + blockIdx.x, s);
+    __stcg(sums + blockIdx.x, s.mid);
+    if constexpr (Doubles) {
+      __stcg(sums + gridDim.x + blockIdx.x, s.big);
+      __stcg(sums + 2 * gridDim.x + blockIdx.x, s.small);
+    }
     __threadfence();
     last = atomicAdd(ticket, 1u) == gridDim.x - 1;
   }
   __syncthreads();
   if (!last) return;
   __threadfence();
-  s = 0;
-  for (int i = threadIdx.x; i < gridDim.x; i += kClipThreads) s += ld_written(sums + i);
-  s = clip_block_sum(s);
+  s = Squares{};
+  for (int i = threadIdx.x; i < gridDim.x; i += kClipThreads) {
+    s.mid += ld_written(sums + i);
+    if constexpr (Doubles) {
+      s.big += ld_written(sums + gridDim.x + i);
+      s.small += ld_written(sums + 2 * gridDim.x + i);
+    }
+  }
+  clip_block_sums(s, Doubles);
   if (threadIdx.x == 0) {
     *ticket = 0u;
-    const double n = sqrt(s), f = max_norm / (n + eps);
+    double n;
+    if constexpr (Doubles) {
+      const bool up = s.big > 0, down = !up && s.mid == 0;
+      n = sqrt(up ? s.big + s.mid * kDown * kDown : down ? s.small : s.mid + s.small * kDown * kDown);
+      n *= up ? kUp : down ? kDown : 1.0;  // what a sum leaves out is below 2^-200 of it
+    } else {
+      n = sqrt(s.mid);
+    }
+    const double f = max_norm / (n + eps);
     *norm = static_cast<float>(n);
-    *factor = n + eps > 0 ? (f > 1.0 ? 1.0 : f) : n == n ? 1.0 : n;  // NaN carries on
+    factor[0] = n + eps > 0 ? (f > 1.0 ? 1.0 : f) : n == n ? 1.0 : n;  // NaN carries on
+    if constexpr (Doubles) {
+      // A factor near fp64's least is divided in two: the values that it leaves
+      // more than 0 are far above those that the first of them would round.
+      const bool split = f < 0x1p-900 && max_norm > 0;
+      if (split) factor[0] = max_norm / ((n + eps) * kDown);
+      factor[1] = split ? kDown : 1.0;
+    }
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void piece_scale(const Piece& c, double factor) {
+// Values times f, in fp32, or in fp64 where fp32 does not hold f (Far).
+template <typename T, bool Far>
+__device__ __forceinline__ void piece_scale(const Piece& c, double f, double first) {
   using Acc = typename AccOf<T>::type;
-  const Acc f = static_cast<Acc>(factor);
+  const Acc g = static_cast<Acc>(f);
+  const auto one = [&](T v) {
+    if constexpr (sizeof(T) == 8) return narrow<T, Acc>(v * first * f);
+    else if constexpr (Far) return narrow<T, Acc>(static_cast<Acc>(static_cast<double>(widen(v)) * f));
+    else return narrow<T, Acc>(widen(v) * g);
+  };
   each_word<T>(
       c,
       [&](uint4* to, const uint4& v) {
         Pack<T, 16> x = as_pack<T>(v);
 #pragma unroll
-        for (int i = 0; i < Pack<T, 16>::N; ++i) x.v[i] = narrow<T, Acc>(widen(x.v[i]) * f);
+        for (int i = 0; i < Pack<T, 16>::N; ++i) x.v[i] = one(x.v[i]);
         __stcs(to, *reinterpret_cast<const uint4*>(&x));
       },
-      [&](T* p) { *p = narrow<T, Acc>(widen(*p) * f); });
+      [&](T* p) { *p = one(*p); });
+}
+
+// Values as large as fp32 holds and a norm beyond make factors that are
+// subnormal in fp32, or 0, and results that are neither.
+constexpr double kFarFactor = 0x1p-100;
+
+// Out of line, as only a step that diverged needs it.
+template <int Only>
+__device__ __noinline__ void scale_far(const Piece* __restrict__ pieces, int count, double f, double first) {
+  for (int c = count - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= gridDim.x) {
+    const Piece q = pieces[c];
+    with_piece<Only>(q, [&](auto tv) {
+      using T = decltype(tv);
+      piece_scale<T, true>(q, sizeof(T) == 8 ? f : f * first, first);
+    });
+  }
 }
 
 template <int Only>
 __global__ void __launch_bounds__(kClipThreads, kClipBlocks / 148)
     scale_pieces(const Piece* __restrict__ pieces, int count, const double* __restrict__ factor) {
-  const double f = *factor;
-  if (f == 1.0) return;
+  const double f = factor[0], first = Only < 0 || Only == SPMVB_F64 ? factor[1] : 1.0, all = f * first;
+  if (all == 1.0) return;
+  if (all > 0 && all < kFarFactor) {
+    scale_far<Only>(pieces, count, f, first);
+    return;
+  }
   for (int c = count - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= gridDim.x) {
     const Piece q = pieces[c];
-    with_piece<Only>(q, [&](auto tv) { piece_scale<decltype(tv)>(q, f); });
+    with_piece<Only>(q, [&](auto tv) {
+      using T = decltype(tv);
+      piece_scale<T, false>(q, sizeof(T) == 8 ? f : all, first);
+    });
   }
 }
 
@@ -251,8 +341,8 @@ spmvb_status spmvb_clip_create(spmvb_context ctx, int32_t count, void* const* h_
       if (h_dtypes[i] != h_dtypes[0]) C->only = -1;
     C->blocks = std::max(1, std::min(C->pieces, kClipBlocks));
     SPMVB_TRY(upload(C->table, pieces.data(), pieces.size() * sizeof(Piece), 16));
-    SPMVB_TRY(C->sums.alloc(static_cast<size_t>(C->blocks) * 8));
-    SPMVB_TRY(C->factor.alloc(8));
+    SPMVB_TRY(C->sums.alloc(static_cast<size_t>(C->blocks) * 3 * 8));
+    SPMVB_TRY(C->factor.alloc(16));
     SPMVB_TRY(C->ticket.alloc(4));
     SPMVB_TRY(scratch_ready());
     C->spans = std::move(spans);
