@@ -77,16 +77,21 @@ struct Words {
   __device__ __forceinline__ Words(const T* row, int w)
       : head(Aligned ? 0 : min(w, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(T)))),
         width(w) {}
-  __device__ __forceinline__ int first(int v) const { return Aligned ? v * N : v == 0 ? 0 : head + (v - 1) * N; }
+  // The last word's first element may lie past the row, and past int32: its
+  // place is an unsigned one, and the count behind it an exact difference.
+  __device__ __forceinline__ int first(int v) const { return static_cast<int>(place(v)); }
   __device__ __forceinline__ int count(int v) const {
     if constexpr (Aligned) return N;
-    return v == 0 ? head : min(N, width - first(v));  // <= 0: past the end
+    return v == 0 ? head : min(N, static_cast<int>(static_cast<unsigned>(width) - place(v)));  // <= 0: past the end
+  }
+  __device__ __forceinline__ unsigned place(int v) const {
+    return Aligned ? static_cast<unsigned>(v) * N : v == 0 ? 0u : head + (static_cast<unsigned>(v) - 1u) * N;
   }
 };
 // Words of a row of any alignment, at most.
 inline int words_of(int width, size_t elem, bool aligned) {
   const int n = static_cast<int>(16 / elem);
-  return aligned ? width / n : (width + n - 1) / n + 1;
+  return aligned ? width / n : (width - 1) / n + 2;
 }
 
 // out[t] = scale * X[idx[t]]. blockDim.x threads share a row and take Ahead

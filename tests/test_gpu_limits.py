@@ -91,3 +91,39 @@ def test_a_timeout_does_not_swallow_the_report_of_an_index(ctx):
         ctx.check()
     assert e.value.status == 1 and "out of range" in str(e.value)
     ctx.check()
+
+
+def test_rows_as_long_as_int32_holds(ctx):
+    """Rows of 2^31 - 1 bf16 values, in every operator that moves rows: the
+    count of their 16-byte words, and the place of the last, pass int32 on the
+    way."""
+    width = 2 ** 31 - 1
+
+    def row(value):
+        return torch.full((1, width), value, dtype=torch.bfloat16, device=DEV)
+
+    one = torch.zeros(1, dtype=torch.int32, device=DEV)
+    x = torch.empty(1, width, dtype=torch.bfloat16, device=DEV).random_(0, 100)
+    y = row(7.0)
+    E = S.Embedding(ctx, 1, width, max_tokens=1)
+    E.lookup(one, x, y)
+    assert torch.equal(x, y)
+    y.fill_(7.0)
+    E.lookup_grad(one, x, y)
+    assert torch.equal(x, y)
+    E.close()
+    R = S.Router(ctx, 4, 1, max_tokens=1)
+    w = torch.ones(1, device=DEV)
+    for call in (R.dispatch, lambda p, a, b: R.dispatch_grad(p, a, b), lambda p, a, b: R.combine(p, w, a, b)):
+        y.fill_(7.0)
+        call(one, x, y)
+        assert torch.equal(x, y)
+    y.fill_(7.0)
+    ones, dw = row(1.0), torch.zeros(1, device=DEV)
+    R.combine_grad(one, w, ones, x, y, dw)
+    assert torch.equal(x, y)
+    # The inner product with ones: the sum of x, each of the block's 256 threads'
+    # terms in order, then a tree of 256.
+    total = x.sum(dtype=torch.float64).item()
+    assert abs(dw.item() - total) <= (width / 8 / 256 + 16) * 2.0 ** -24 * total
+    ctx.check()
