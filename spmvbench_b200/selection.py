@@ -36,6 +36,15 @@ def _torch_names() -> None:
         lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
+def _int32(v, what: str) -> int:
+    """An integer for the C side, which would take what int32 does not hold
+    modulo 2^32."""
+    n = _as_int(v)
+    if not -_MOST - 1 <= n <= _MOST:
+        raise ValueError(f"{what} = {n} does not fit int32")
+    return n
+
+
 def _stream(stream, device: int) -> int:
     if stream is None:
         return _raw_stream(device)
@@ -72,7 +81,7 @@ def _rows(t, rows, width: int, device: int, what: str, codes=(F32, F16, BF16)):
     stride; returns (dtype code, row stride, address)."""
     code = _code(t, codes, device, what)
     shape = t.shape
-    if len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows) or shape[0] > _MOST:
+    if len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows) or shape[0] > _MOST or width > _MOST:
         raise ValueError(f"{what} has shape {tuple(shape)}; ({'any' if rows is None else rows}, {width}) is needed")
     ld, unit = t.stride()
     if unit != 1 or ld < width:
@@ -120,6 +129,7 @@ class Embedding(_Handle):
     _destroy = "spmvb_embedding_destroy"
 
     def __init__(self, ctx, rows: int, width: int, max_tokens: int):
+        rows, width, max_tokens = _int32(rows, "rows"), _int32(width, "width"), _int32(max_tokens, "max_tokens")
         h = C.c_void_p()
         call("spmvb_embedding_create", ctx.handle, rows, width, max_tokens, C.byref(h))
         self.handle, self.ctx = h, ctx
@@ -161,10 +171,11 @@ class Router(_Handle):
     def __init__(self, ctx, experts: int, k: int, max_tokens: int, score: str = "softmax", renormalise: bool = True,
                  scale: float = 1.0, groups: int = 1, groups_kept: int | None = None, group_top: int = 1):
         spec = router_spec(experts, k, score, renormalise, scale, groups, groups_kept, group_top)
+        max_tokens = _int32(max_tokens, "max_tokens")
         h = C.c_void_p()
         call("spmvb_router_create", ctx.handle, C.byref(spec), max_tokens, C.byref(h))
         self.handle, self.ctx = h, ctx
-        self.experts, self.k, self.max_tokens = experts, k, max_tokens
+        self.experts, self.k, self.max_tokens = spec.experts, spec.k, max_tokens
 
     def route(self, logits, indices, weights, bias=None, offsets=None, order=None, position=None, stream=None) -> None:
         """The chosen experts of each row of logits (tokens x experts), best
@@ -263,8 +274,8 @@ def router_spec(experts: int, k: int, score: str = "softmax", renormalise: bool 
     if score not in SCORES:
         raise ValueError(f"score must be one of {sorted(SCORES)}")
     kept = groups if groups_kept is None else groups_kept
-    spec = _lib.RouterSpec(_as_int(experts), _as_int(k), SCORES[score], int(bool(renormalise)), _as_int(groups),
-                           _as_int(kept), _as_int(group_top), scale)
+    spec = _lib.RouterSpec(_int32(experts, "experts"), _int32(k, "k"), SCORES[score], int(bool(renormalise)),
+                           _int32(groups, "groups"), _int32(kept, "groups_kept"), _int32(group_top, "group_top"), scale)
     call("spmvb_router_check", C.byref(spec))
     return spec
 
