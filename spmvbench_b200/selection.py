@@ -283,27 +283,45 @@ def router_spec(experts: int, k: int, score: str = "softmax", renormalise: bool 
 class GradClip(_Handle):
     """The 2-norm over all of `tensors`, and their scaling in place by
     min(1, max_norm / (norm + eps)) (spmvb_clip). float32, float16, bfloat16
-    and float64, contiguous, none overlapping another. The handle keeps the
-    tensors; a tensor whose storage has been replaced since is refused."""
+    and float64, contiguous, none overlapping another.
+
+    The handle keeps the tensors and works on their memory: they have to keep
+    their storage (a replaced one is refused) and their sizes. A parameter's
+    gradient is another tensor after zero_grad(set_to_none=True), which is
+    torch's default: the handle then still holds the old ones, which nobody
+    else does. Zero gradients in place, or make a new handle. With
+    `parameters`, the tensors' owners, one each, a call is refused where a
+    parameter's .grad is no longer its tensor."""
 
     _destroy = "spmvb_clip_destroy"
 
-    def __init__(self, ctx, tensors):
+    def __init__(self, ctx, tensors, parameters=None):
         tensors = list(tensors)
+        owners = [] if parameters is None else list(parameters)
+        if parameters is not None and len(owners) != len(tensors):
+            raise ValueError(f"{len(tensors)} tensors of {len(owners)} parameters")
         dev, codes = ctx.device, []
         for i, t in enumerate(tensors):
             codes.append(_code(t, _ALL, dev, f"tensor {i}"))
             if not t.is_contiguous():
                 raise ValueError(f"tensor {i} must be contiguous")
         n = len(tensors)
-        self._tensors, self._places = tensors, [t.data_ptr() for t in tensors]
+        self._tensors, self._places, self._owners = tensors, [t.data_ptr() for t in tensors], owners
+        self._check_owners()
         h = C.c_void_p()
         call("spmvb_clip_create", ctx.handle, n, (C.c_void_p * n)(*self._places),
              (C.c_int64 * n)(*[t.numel() for t in tensors]), (C.c_int * n)(*codes),
              C.byref(h))
         self.handle, self.ctx = h, ctx
 
+    def _check_owners(self) -> None:
+        for i, (p, t) in enumerate(zip(self._owners, self._tensors)):
+            if p.grad is not t:
+                raise ValueError(f"the gradient of parameter {i} is another tensor: make a new GradClip")
+
     def _check(self, norm) -> int:
+        if self._owners:
+            self._check_owners()
         if [t.data_ptr() for t in self._tensors] != self._places:
             raise ValueError("a tensor's storage has been replaced: make a new GradClip")
         return _flat(norm, F32, 1, self.ctx.device, "norm")
