@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import spmvbench_b200 as S
-from selection_util import choose
+from selection_util import check, choose, plan_of, weights_of
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +87,84 @@ def test_a_lone_choice_has_the_whole_weight(ctx, tokens, score, dtype):
         R = S.Router(ctx, 64, k, max_tokens=tokens, score=score, scale=2.5)
         R.route_grad(logits.to(DEV), indices.to(DEV), torch.randn(tokens, k, generator=g).to(DEV), d)
         assert not d.any()
+
+
+# ---- rows that share a warp ------------------------------------------------------
+
+def weight_error(logits, picks, score, renormalise, experts):
+    """fp32's error of a row's weights, relative, u = 2^-24 a rounding. exp has
+    2 u and u a unit of its argument (a difference of two logits, `reach` at
+    most); a quotient 4 u; a scale 1 u.
+    - renormalised: two such exps, under the sigmoid each over 1 + exp (5 + 4
+      u), up to 32 values summed in a tree (5 u), a quotient, the scale.
+    - sigmoid: exp, 1 +, quotient, scale.
+    - softmax: exp over the row's sum, whose exps are rougher (4 u, and 2 u a
+      unit: the argument times log2 e) and are added 64 one after the other at
+      most and 5 in a tree."""
+    l = logits.double()
+    if renormalise:
+        l = torch.where(picks >= 0, l.gather(1, picks.clamp(min=0).long()), math.nan)
+        if score == "sigmoid":
+            l = l.clamp(max=0)
+    elif score == "sigmoid":
+        return torch.full((l.shape[0], 1), 12 * 2.0 ** -24, dtype=torch.float64)
+    there = (l > -math.inf) & (l < math.inf)
+    reach = torch.where(there, l, -1e30).amax(1, keepdim=True) - torch.where(there, l, 1e30).amin(1, keepdim=True)
+    # Past 120 below the largest a weight is 0 in fp32, and its error absolute.
+    reach = torch.where(there.any(1, keepdim=True), reach, 0.0).clamp(0, 120)
+    return (2 * reach + 24 if renormalise else 3 * reach + 16 + experts / 8) * 2.0 ** -24
+
+
+SHARED = [
+    # experts, k, score, renormalise, groups, kept, top, bias
+    (16, 2, "softmax", True, 1, 1, 1, False), (16, 8, "sigmoid", False, 4, 2, 2, True), (60, 4, "softmax", False, 1, 1, 1, False),
+    (60, 4, "sigmoid", True, 5, 3, 1, False), (64, 8, "softmax", True, 1, 1, 1, False), (64, 6, "sigmoid", True, 8, 3, 2, True),
+    (64, 2, "softmax", False, 8, 2, 1, False), (64, 8, "softmax", False, 8, 4, 2, False), (100, 10, "softmax", True, 1, 1, 1, True),
+    (100, 6, "sigmoid", False, 4, 2, 2, False), (128, 16, "sigmoid", True, 16, 8, 2, True), (128, 8, "softmax", False, 1, 1, 1, False),
+    (96, 12, "softmax", True, 4, 2, 1, False), (3, 1, "sigmoid", False, 1, 1, 1, False), (256, 8, "sigmoid", True, 8, 4, 2, True)]
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("experts,k,score,renormalise,groups,kept,top,bias", SHARED)
+def test_rows_that_share_a_warp(ctx, experts, k, score, renormalise, groups, kept, top, bias, dtype):
+    """A training batch (1,301 rows, of which four or two share a warp):
+    choices, weights and plan, with masks, equal logits, and rows of NaN and
+    infinities beside ordinary ones."""
+    tokens = 1301
+    g = torch.Generator().manual_seed(experts * 3 + k)
+    l = torch.randn(tokens, experts, generator=g) * 2
+    l = torch.where(torch.rand(tokens, 1, generator=g) < 0.3, (l * 2).round() / 2, l)
+    l = torch.where(torch.rand(tokens, experts, generator=g) < 0.1, -math.inf, l)
+    l[torch.rand(tokens, generator=g) < 0.05] = -math.inf
+    for v in (math.nan, math.inf, torch.finfo(dtype).min):
+        l = torch.where((torch.rand(tokens, experts, generator=g) < 0.3) & (torch.rand(tokens, 1, generator=g) < 0.04), v, l)
+    l[7] = math.nan
+    l = l.to(dtype)
+    b = (torch.randn(experts, generator=g) * 0.1) if bias else None
+    spec = dict(score=score, renormalise=renormalise, scale=2.5, groups=groups, groups_kept=kept, group_top=top)
+    R = S.Router(ctx, experts, k, max_tokens=tokens, **spec)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    indices, weights = torch.full((tokens, k), 77, **i32), torch.full((tokens, k), 77.0, device=DEV)
+    offsets, order, position = torch.full((experts + 1,), 77, **i32), torch.full((tokens * k,), -77, **i32), torch.full((tokens, k), 77, **i32)
+    wide = torch.full((tokens, experts + 3), math.nan, device=DEV, dtype=dtype)
+    wide[:, :experts] = l.to(DEV)
+    picks = choose(l, b, k, score, groups, kept, top)
+    none = (torch.isnan(l) | (l == math.inf)).any(1, keepdim=True) if score == "softmax" else torch.zeros(tokens, 1, dtype=torch.bool)
+    ref = torch.where(none, math.nan, weights_of(l, picks, score, renormalise, 2.5))
+    bound = ref.nan_to_num().abs() * weight_error(l, picks, score, renormalise, experts) + 2.0 ** -120
+    # Rows of a wider buffer, then rows that 16-byte words fit; with the plan, then without.
+    for logits in (wide[:, :experts], l.to(DEV)):
+        R.route(logits, indices, weights, bias=None if b is None else b.to(DEV), offsets=offsets, order=order, position=position)
+        assert torch.equal(indices.cpu(), picks)
+        check(weights, ref, bound, "weights")
+        o, by, at = plan_of(picks, experts)
+        assert offsets.tolist() == o and position.flatten().tolist() == at and order[:len(by)].tolist() == by
+        again, w2 = route(ctx, logits, k, bias=b, **spec)
+        assert torch.equal(again, picks) and torch.equal(w2.view(torch.int32), weights.cpu().view(torch.int32))
+    # Every row alone chooses the same.
+    some = list(range(0, tokens, 37)) + [7]
+    for t in some:
+        i, w = route(ctx, l[t:t + 1], k, bias=b, **spec)
+        assert torch.equal(i[0], picks[t])
+        check(w, ref[t:t + 1], bound[t:t + 1], "weights of a row alone")
+    ctx.check()
