@@ -127,3 +127,32 @@ def test_rows_as_long_as_int32_holds(ctx):
     total = x.sum(dtype=torch.float64).item()
     assert abs(dw.item() - total) <= (width / 8 / 256 + 16) * 2.0 ** -24 * total
     ctx.check()
+
+
+@pytest.mark.parametrize("code", [S.F16, S.BF16])
+def test_matrices_refuse_16_bit_types_for_their_type(ctx, code):
+    """Every entry point of the sparse matrices that takes a type, with all
+    other arguments in order."""
+    A = S.generate(2, seed=1, scale_rows=64)
+    lib, out = S.load(), C.c_void_p()
+    at_host = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
+    refused(lib.spmvb_matrix_create_csr(ctx.handle, code, A.m, A.n, A.nnz, at_host(A.rowptr), at_host(A.colind), at_host(A.values),
+                                        C.byref(out)), "bad dtype")
+    bounds = S.partition_rows(A.rowptr, 1)
+    refused(lib.spmvb_dist_create(ctx.handle, 1, 0, None, code, A.m, A.nnz, at_host(A.rowptr), at_host(A.colind),
+                                  at_host(A.values), at_host(bounds), C.byref(out)), "bad dtype")
+    M = S.DeviceMatrix(ctx, A, S.F32)
+    x, y = torch.zeros(A.n * 4, device=DEV), torch.zeros(A.m * 4, device=DEV)
+    hx, hy, ms = S.generate_vector(1, A.n * 4).astype("float32"), S.generate_vector(2, A.m * 4), (C.c_double * 4)()
+    h, k = M.handle, S.CSR_SCALAR
+    for status in (lambda: lib.spmvb_spmv(h, k, 0, 0, at(x), at(y), code, None),
+                   lambda: lib.spmvb_spmv_host(h, k, 0, 0, at_host(hx), at_host(hy), code, None),
+                   lambda: lib.spmvb_spmv_time(h, k, 0, 0, at(x), at(y), code, 1, 0, None, ms),
+                   lambda: lib.spmvb_spmm(h, 32, 0, 4, at(x), at(y), code, None),
+                   lambda: lib.spmvb_spmm_host(h, 32, 0, 4, at_host(hx), at_host(hy), code, None)):
+        refused(status(), "bad accumulator dtype")
+    P = C.c_void_p()
+    assert lib.spmvb_pipeline_create(h, 2, C.byref(P)) == 0
+    refused(lib.spmvb_pipeline_submit(P, k, 0, 0, at_host(hx), at_host(hy), code), "bad accumulator dtype")
+    assert lib.spmvb_pipeline_destroy(P) == 0
+    M.close()

@@ -46,3 +46,13 @@ class Wide:
 def test_rows_longer_than_int32_are_refused():
     with pytest.raises(ValueError, match="shape"):
         selection._rows(Wide(), 1, 2 ** 32 + 16, 0, "X")
+
+
+@pytest.mark.parametrize("code", [S.F16, S.BF16])
+def test_the_merge_product_refuses_16_bit_types_for_their_type(code):
+    """An empty product, which every other argument allows."""
+    lib = S.load()
+    empty = lambda dtype, acc: lib.spmvb_spmv_merge_noalloc(dtype, 0, 0, 0, None, None, None, None, None, acc, None)  # noqa: E731
+    assert empty(S.F32, S.F32) == 0 and empty(S.F32, S.F64) == 0
+    assert empty(code, S.F32) == 1 and lib.spmvb_last_error() == b"bad dtype"
+    assert empty(S.F32, code) == 1 and lib.spmvb_last_error() == b"bad accumulator dtype"
