@@ -157,6 +157,8 @@ spmvb_status spmvb_query_gpu(int device, spmvb_gpu_info* out);
 /* A context binds one device. Replaces the implicit current-device state the
  * reference's SpmvRunner relies on (src/cuda/spmv_cuda.cu:233-290). */
 spmvb_status spmvb_context_create(int device, spmvb_context* out);
+/* Handles made from the context stay usable and keep what they need of it;
+ * their kernels' reports can then no longer be asked for. */
 spmvb_status spmvb_context_destroy(spmvb_context ctx);
 /* Synchronizes the device and reports whether any kernel launched through
  * this context gave up a bounded wait since the last check

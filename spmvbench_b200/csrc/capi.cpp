@@ -236,7 +236,7 @@ spmvb_status spmvb_context_destroy(spmvb_context ctx) {
   clear_error();
   if (ctx) {
     DeviceGuard g(ctx->device);
-    delete ctx;
+    ctx->release();
   }
   return SPMVB_OK;
 }
@@ -272,7 +272,7 @@ spmvb_status spmvb_matrix_create_csr(spmvb_context ctx, spmvb_dtype dtype, int32
   if (nnz > 0 && !h_values) return fail(SPMVB_ERR_INVALID_ARGUMENT, "null values");
   DeviceGuard g(ctx->device);
   auto* A = new spmvb_matrix_st;
-  A->ctx = ctx;
+  A->ctx.hold(ctx);
   A->device = ctx->device;
   A->dtype = dtype;
   A->m = m;

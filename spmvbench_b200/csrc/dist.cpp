@@ -38,7 +38,7 @@
 using namespace spmvb;
 
 struct spmvb_dist_st {
-  spmvb_context ctx = nullptr;
+  ContextRef ctx;
   int nranks = 1;
   int rank = 0;
   spmvb_dtype dtype = SPMVB_F64;
@@ -228,7 +228,7 @@ spmvb_status spmvb_dist_create(spmvb_context ctx, int nranks, int rank, const vo
     if (h_bounds[g + 1] < h_bounds[g]) return fail(SPMVB_ERR_INVALID_ARGUMENT, "bounds must be non-decreasing");
   DeviceGuard guard(ctx->device);
   auto D = std::make_unique<spmvb_dist_st>();
-  D->ctx = ctx;
+  D->ctx.hold(ctx);
   D->nranks = nranks;
   D->rank = rank;
   D->dtype = dtype;

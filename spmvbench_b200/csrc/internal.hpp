@@ -112,10 +112,41 @@ struct spmvb_context_st {
   // (see spmvb_context_check).
   spmvb::DevBuf err;
   int* index_err() const { return err.as<int>() + 1; }
+  // The caller's reference and one of each handle made from the context, whose
+  // kernels write to the error words: the last one to go frees them.
+  std::atomic<int> refs{1};
+  void release() {
+    if (refs.fetch_sub(1) == 1) delete this;
+  }
 };
 
+namespace spmvb {
+
+// A handle's reference to its context.
+class ContextRef {
+ public:
+  ContextRef() = default;
+  ~ContextRef() {
+    if (p_) p_->release();
+  }
+  ContextRef(const ContextRef&) = delete;
+  ContextRef& operator=(const ContextRef&) = delete;
+  void hold(spmvb_context ctx) {
+    ctx->refs.fetch_add(1);
+    if (p_) p_->release();
+    p_ = ctx;
+  }
+  spmvb_context operator->() const { return p_; }
+  operator spmvb_context() const { return p_; }
+
+ private:
+  spmvb_context p_ = nullptr;
+};
+
+}  // namespace spmvb
+
 struct spmvb_matrix_st {
-  spmvb_context ctx = nullptr;
+  spmvb::ContextRef ctx;
   int device = 0;
   spmvb_dtype dtype = SPMVB_F64;
   int m = 0;

@@ -801,7 +801,7 @@ spmvb_status with_logits(spmvb_dtype d, int slots, F&& f) {
 }  // namespace spmvb
 
 struct spmvb_router_st {
-  spmvb_context ctx = nullptr;
+  spmvb::ContextRef ctx;
   spmvb_router_spec spec{};
   int device = 0, max_tokens = 0;
   spmvb::PlanSpace plan;
@@ -877,7 +877,7 @@ spmvb_status spmvb_router_create(spmvb_context ctx, const spmvb_router_spec* spe
   return constructed([&]() -> spmvb_status {
     DeviceGuard g(ctx->device);
     auto R = std::make_unique<spmvb_router_st>();
-    R->ctx = ctx;
+    R->ctx.hold(ctx);
     R->device = ctx->device;
     R->spec = *spec;
     R->max_tokens = max_tokens;

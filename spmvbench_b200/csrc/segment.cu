@@ -974,7 +974,7 @@ spmvb_status order_tokens_by_row(SortSpace& space, const int* idx, int count, in
 }  // namespace spmvb
 
 struct spmvb_embedding_st {
-  spmvb_context ctx = nullptr;
+  spmvb::ContextRef ctx;
   int device = 0, rows = 0, width = 0, max_tokens = 0;
   int64_t chunks = 0;  // that parts and tickets are for
   spmvb::SortSpace sort;
@@ -1067,7 +1067,7 @@ spmvb_status spmvb_embedding_create(spmvb_context ctx, int32_t rows, int32_t wid
   return constructed([&]() -> spmvb_status {
     DeviceGuard g(ctx->device);
     auto E = std::make_unique<spmvb_embedding_st>();
-    E->ctx = ctx;
+    E->ctx.hold(ctx);
     E->device = ctx->device;
     E->rows = rows;
     E->width = width;
