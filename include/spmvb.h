@@ -515,9 +515,11 @@ spmvb_status spmvb_dist_pipeline_destroy(spmvb_dist_pipeline P);
  *  - dtype is SPMVB_F32, F16 or BF16; the embedding and gradient clipping
  *    take SPMVB_F64 too. Sums are held in fp32 (fp64 for F64) and rounded
  *    once.
- *  - ld_* are row strides in elements, at least the row's length. Rows whose
- *    addresses and length are multiples of 16 bytes are moved 16 bytes at a
- *    time, others in smaller pieces.
+ *  - ld_* are row strides in elements, at least the row's length. Rows may
+ *    have any alignment; fastest are those whose addresses and lengths are
+ *    multiples of 16 bytes. Lookup and exchange move others in 16-byte words
+ *    put together from two, the embedding's gradient in accesses of the size
+ *    that their alignment allows.
  *  - A negative index selects nothing: a zero row, or no contribution. An
  *    index past the end is left out in the same way and reported by
  *    spmvb_context_check. Positions (of the experts' rows) are distinct, as
@@ -530,7 +532,11 @@ spmvb_status spmvb_dist_pipeline_destroy(spmvb_dist_pipeline P);
  *  - Results do not depend on timing: sums have a fixed order. */
 typedef struct spmvb_embedding_st* spmvb_embedding;
 /* Scratch for the gradient of up to max_tokens rows of a rows x width table:
- * about max_tokens * width bytes, and an eighth of a byte a row. */
+ * max_tokens * width bytes or, if that is more, 4 * min(max_tokens, few) * width
+ * (few = SMs * 4096 / t: how many tokens are added up in small chunks; t is
+ * the least power of two, 8 to 256, of at least an eighth of the width), 18 bytes
+ * a token for their order, 3 bytes a token per 256 columns at most, and an
+ * eighth of a byte a table row. Lookups need none (max_tokens = 0). */
 spmvb_status spmvb_embedding_create(spmvb_context ctx, int32_t rows,
                                     int32_t width, int32_t max_tokens,
                                     spmvb_embedding* out);

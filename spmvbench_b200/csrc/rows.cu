@@ -7,9 +7,14 @@
 //   combine        out[t]          = sum_j w[t,j] * Y[pos[t,j]]
 //   combine_grad   dY[pos[t,j]]    = w[t,j] * dout[t],  dw[t,j] = <dout[t], Y[pos[t,j]]>
 //
-// Each is one pass over its rows: every row is read once and written once,
-// so HBM bounds all of them. Sums over j run in order in fp32 (fp64 for
-// doubles) and are rounded once.
+// Each is one pass over its rows. Sums over j run in order in fp32 (fp64 for
+// doubles) and are rounded once. Where rows begin and end on 16-byte words every
+// row is read once and written once, and HBM bounds them: about 0.9 of the copy rate
+// for rows of 8 KB. Other rows take 2.3 to 3.7 times their floor, for the two
+// loads a word, the ends moved by element, and dispatch reading a row again for
+// each of its places: the lookup of 16,384 rows of 1,001 bf16 values 22.6 us
+// (floor 8.0), dispatch + combine of 3,001 tokens x 3 such rows 27 us (7.2), both
+// gradients in fp32 45.7 us (19.9).
 //
 // Rows are moved in 16-byte words of the row that is written. Where every row
 // begins on such a word (Aligned), the words of the rows read are the same;
