@@ -248,14 +248,20 @@ spmvb_status spmvb_context_check(spmvb_context ctx) {
   SPMVB_TRY_CUDA(cudaDeviceSynchronize());
   int code[2] = {0, 0};
   SPMVB_TRY_CUDA(cudaMemcpy(code, ctx->err.get(), sizeof(code), cudaMemcpyDeviceToHost));
-  // Only the word that is reported is cleared: the other one waits for the
-  // next check.
+  // Only the word that is reported is cleared (the other one waits for the next
+  // check), and before the return: streams that do not wait for the legacy one
+  // may report anew right after it.
+  const auto clear = [](int* word) -> spmvb_status {
+    SPMVB_TRY_CUDA(cudaMemset(word, 0, sizeof(int)));
+    SPMVB_TRY_CUDA(cudaStreamSynchronize(nullptr));
+    return SPMVB_OK;
+  };
   if (code[0] != 0) {
-    SPMVB_TRY_CUDA(cudaMemset(ctx->err.get(), 0, sizeof(int)));
+    SPMVB_TRY(clear(ctx->err.as<int>()));
     return fail(SPMVB_ERR_TIMEOUT, "a kernel's bounded wait gave up (device error code " + std::to_string(code[0]) + ")");
   }
   if (code[1] != 0) {
-    SPMVB_TRY_CUDA(cudaMemset(ctx->index_err(), 0, sizeof(int)));
+    SPMVB_TRY(clear(ctx->index_err()));
     return fail(SPMVB_ERR_INVALID_ARGUMENT, "a row-selection operator met an index out of range and left it out");
   }
   return SPMVB_OK;

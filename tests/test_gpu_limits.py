@@ -156,3 +156,21 @@ def test_matrices_refuse_16_bit_types_for_their_type(ctx, code):
     refused(lib.spmvb_pipeline_submit(P, k, 0, 0, at_host(hx), at_host(hy), code), "bad accumulator dtype")
     assert lib.spmvb_pipeline_destroy(P) == 0
     M.close()
+
+
+def test_reports_right_after_a_check_are_kept(ctx):
+    """An index past the end on a stream that does not wait for the default
+    one, enqueued as soon as a check that cleared the last report returns."""
+    E = S.Embedding(ctx, 4, 8, max_tokens=1)
+    side = torch.cuda.Stream()
+    table, out = torch.ones(4, 8, device=DEV), torch.zeros(1, 8, device=DEV)
+    bad = torch.full((1,), 9, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    E.lookup(bad, table, out, stream=side)
+    for turn in range(200):
+        with pytest.raises(S.SpmvbError):
+            ctx.check()
+        E.lookup(bad, table, out, stream=side)
+    with pytest.raises(S.SpmvbError):
+        ctx.check()
+    ctx.check()
